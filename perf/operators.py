@@ -128,9 +128,6 @@ def _bucket_of(distance, buckets, max_distance, causal):
 
 
 def _bucket_map(case):
-    if own:
-        from recboard_amd import ops
-        return ops.relative_buckets(case["buckets"], case["distance"], bidirectional=not case["causal"], device="cuda")
     far = case["distance"]
     return torch.tensor([_bucket_of(d, case["buckets"], far, case["causal"]) for d in range(-far, far + 1)], dtype=torch.int32, device="cuda")
 
@@ -250,9 +247,17 @@ def _bucket_ids(bucket_map, queries, keys, offset):
     return bucket_map[at.clamp(-far, far) + far].long()
 
 
-def _sum_by_bucket(d, ids, buckets):
-    """[buckets, heads] sums of d [heads, queries, keys]."""
-    return torch.stack([torch.where(ids == k, d, 0.0).sum(dim=(1, 2), dtype=torch.float64) for k in range(buckets)])
+def _sum_by_bucket(d, bucket_map, buckets, offset):
+    """[buckets, heads] sums of d [heads, queries, keys]: along the diagonals first (a row is one longer than the row that it is read back
+    in, so that row i moves i places), then the diagonals of a bucket."""
+    heads, queries, keys = d.shape
+    sheared = torch.nn.functional.pad(d.flip(1), (0, queries)).reshape(heads, -1)[:, :-queries].reshape(heads, queries, queries + keys - 1)
+    along = sheared.sum(dim=1, dtype=torch.float64)                       # column c: key - query = c - (queries - 1)
+    far = bucket_map.numel() // 2
+    at = torch.arange(queries + keys - 1, device=d.device) - (queries - 1) - offset
+    ids = bucket_map[at.clamp(-far, far) + far].long()
+    member = (ids.unsqueeze(1) == torch.arange(buckets, device=d.device)).double()
+    return torch.matmul(along, member).t()
 
 
 def _bias_plain(case, s):
@@ -260,7 +265,7 @@ def _bias_plain(case, s):
     ids = _bucket_ids(s["map"], queries, keys, keys - queries)
     t = s["table"].dtype
     bias = s["table"].t()[:, ids]
-    return {"bias": bias, "dtable": _sum_by_bucket(s["dbias"].float(), ids, case["buckets"]).to(t)}
+    return {"bias": bias, "dtable": _sum_by_bucket(s["dbias"].float(), s["map"], case["buckets"], keys - queries).to(t)}
 
 
 def _attention_own(case, s):
@@ -327,7 +332,7 @@ def _attention_plain(case, s):
     dp = rows(torch.matmul(dout, v.transpose(2, 3).contiguous()))
     ds = p * (dp - (p * dp).sum(dim=3, keepdim=True))
     if case["buckets"]:
-        r["dtable"] = _sum_by_bucket(ds.sum(dim=0), ids, case["buckets"]).to(t)
+        r["dtable"] = _sum_by_bucket(ds.sum(dim=0), s["map"], case["buckets"], keys - queries).to(t)
     ds = ds.reshape(batch, kv_heads, group * queries, keys)
     r["dq"] = rows(torch.matmul(ds, k) * scale).to(t)
     r["dk"] = (torch.matmul(ds.transpose(2, 3).contiguous(), q) * scale).to(t)
