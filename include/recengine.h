@@ -716,6 +716,39 @@ int re_bn_bwd_apply(float* g, const float* z, int64_t M, int64_t N, const float*
 /* dst[i] = alpha * src[i]  (LightGCN/main.py:80 `avgEmbds = allEmbds / (L+1)`) */
 int re_scale_copy(float* dst, const float* src, float alpha, int64_t n, re_stream_t stream);
 
+/* =========================================================================================================
+ * Operators of a transformer block: layer norm, the relative position bias by buckets, attention.  Their tensors are fp32, bf16 or
+ * fp16 (one type per call, RE_F32 / RE_BF16 / RE_F16); all statistics, softmax sums and gradient sums are held in fp32.
+ * Run to run the same bits (no atomics). */
+#define RE_F32 0
+#define RE_BF16 1
+#define RE_F16 2
+
+/* Layer norm over the last dimension of x [rows, D] (contiguous, 1 <= D <= 2^24), alone or behind a residual sum:
+ *   s = x + residual (residual may be NULL),  y = (s - mean) / sqrt(var + eps) * weight + bias
+ * weight / bias [D] of type `wtype`, either may be NULL (1 / 0).  sum (may be NULL) receives s rounded to `dtype`; mean / rstd [rows]
+ * (may be NULL) what the backward needs.  Replaces the elementwise chains of FMLP-Rec/modules.py:27-40 and torch.nn.LayerNorm at
+ * BERT4Rec/main.py:60, BSARec/modules.py:95. */
+int re_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows, int64_t D, float eps,
+                      int32_t dtype, int32_t wtype, void* y, void* sum, float* mean, float* rstd, re_stream_t stream);
+/* Its backward: dx [rows, D] = the gradient of s (= of x and of residual), `dsum` (may be NULL) the gradient that reaches s on another
+ * way, added in; dweight / dbias [D] of type `wtype` (either may be NULL).  s: x of a call without residual, else its `sum`. */
+size_t re_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D);
+int re_layer_norm_bwd(const void* dy, const void* s, const void* weight, const float* mean, const float* rstd, const void* dsum,
+                      int64_t rows, int64_t D, int32_t dtype, int32_t wtype, void* dx, void* dweight, void* dbias, void* ws,
+                      size_t ws_bytes, re_stream_t stream);
+
+/* Relative position bias by buckets: bias[h, i, j] = table[bucket_map[clip(j - (i + offset), -R, R) + R], h], R = max_distance,
+ * bucket_map [2 R + 1] DEVICE int32, table [buckets, H]; an entry of the map outside [0, buckets) reads as 0 and takes no gradient.
+ * R <= 1024, buckets <= 256, H <= 65535, Sq <= 2^27 (RE_EUNSUPPORTED / RE_EINVAL beyond).
+ * _bwd: dtable[k, h] (type `table_dtype`) = sum of dbias [H, Sq, Sk] (type `dtype`, contiguous) over the pairs in bucket k. */
+int re_relative_bias_fwd(const void* table, const int32_t* bucket_map, int64_t buckets, int64_t max_distance, int64_t H, int64_t Sq,
+                         int64_t Sk, int64_t offset, int32_t dtype, void* bias, re_stream_t stream);
+size_t re_relative_bias_bwd_workspace_bytes(int64_t H, int64_t Sq, int64_t buckets);
+int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t buckets, int64_t max_distance, int64_t H, int64_t Sq,
+                         int64_t Sk, int64_t offset, int32_t dtype, void* dtable, int32_t table_dtype, void* ws, size_t ws_bytes,
+                         re_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

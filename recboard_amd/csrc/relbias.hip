@@ -1,0 +1,163 @@
+// Relative position bias by buckets, materialised, and its gradient.
+//
+//   bias[h, i, j] = table[map[clip(j - (i + offset), -R, R) + R], h]        R = max_distance, map [2 R + 1]
+//   dtable[k, h]  = sum of dbias[h, i, j] over the pairs whose clipped distance lies in bucket k
+//
+// Bound by HBM: H Sq Sk elements written, or read, once.  Forward: the 2 R + 1 values of a head sit in LDS and a lane looks up the VEC elements of
+// one 16-byte store.  Backward: a lane owns DIAGONALS inside the band |j - i - offset| < R -- its column moves with the row, so the sum of a
+// diagonal stays in one register -- while the two clipped sides (one bucket each) are summed with 16-byte loads.  A workgroup's diagonals are
+// then added into its buckets and the workgroups' buckets by a second launch, in a fixed order.
+#include "relbias.h"
+
+namespace {
+
+constexpr int RB_ROWS = 16;       // query rows of a workgroup
+
+struct rb_args {
+    const void* in;               // table / dbias
+    void* out;                    // bias  / partial buckets
+    const int32_t* map;
+    int64_t H, Sq, Sk, offset;
+    int32_t R, buckets;
+};
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void rb_fwd_k(const rb_args a) {
+    __shared__ T line[2 * RB_MAX_DISTANCE + 1];
+    const int64_t h = blockIdx.y, i0 = (int64_t)blockIdx.x * RB_ROWS;
+    for (int d = threadIdx.x; d < 2 * a.R + 1; d += 256) {
+        const int k = a.map[d];
+        line[d] = (unsigned)k < (unsigned)a.buckets ? static_cast<const T*>(a.in)[k * a.H + h] : (T)0.f;
+    }
+    __syncthreads();
+    const int64_t nv = (a.Sk + VEC - 1) / VEC;
+    const int rows = (int)min((int64_t)RB_ROWS, a.Sq - i0);
+    // lanes run over (row, piece): short rows share a pass
+    for (int64_t t = threadIdx.x; t < rows * nv; t += 256) {
+        const int64_t row = t / nv, j = (t - row * nv) * VEC, i = i0 + row;
+        const int64_t base = j - i - a.offset;
+        re_vec<T, VEC> v;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const int64_t d = base + e;
+            v.e[e] = line[(d < -a.R ? -a.R : d > a.R ? a.R : (int)d) + a.R];
+        }
+        *reinterpret_cast<re_vec<T, VEC>*>(static_cast<T*>(a.out) + (h * a.Sq + i) * a.Sk + j) = v;
+    }
+}
+
+template <class T, int VEC>
+__global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
+    constexpr int MAXD = (2 * RB_MAX_DISTANCE + 1 + 255) / 256;
+    __shared__ float line[2 * RB_MAX_DISTANCE + 1];
+    __shared__ float tmp[256];
+    const int64_t h = blockIdx.y, i0 = (int64_t)blockIdx.x * RB_ROWS;
+    const int R = a.R, band = 2 * R - 1;              // distances -(R - 1) .. R - 1
+    float acc[MAXD];
+#pragma unroll
+    for (int m = 0; m < MAXD; ++m) acc[m] = 0.f;
+    float left = 0.f, right = 0.f;
+    const int64_t nv = a.Sk / VEC;                    // (VEC > 1 only where it divides Sk)
+    const int64_t i1 = min(i0 + RB_ROWS, a.Sq);
+    for (int64_t i = i0; i < i1; ++i) {
+        const T* g = static_cast<const T*>(a.in) + (h * a.Sq + i) * a.Sk;
+        const int64_t lo = i + a.offset - R, hi = i + a.offset + R;      // columns <= lo and >= hi are clipped
+        for (int64_t t = threadIdx.x; t < nv; t += 256) {
+            const int64_t j = t * VEC;
+            if (j > lo && j + VEC - 1 < hi) continue;
+            float f[VEC];
+            re_load_vec<T, VEC>(g + j, f);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                left += j + e <= lo ? f[e] : 0.f;
+                right += j + e >= hi ? f[e] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int m = 0; m < MAXD; ++m) {
+            if (m * 256 >= band) break;
+            const int d = m * 256 + threadIdx.x;
+            const int64_t j = lo + 1 + d;
+            if (d < band && j >= 0 && j < a.Sk) acc[m] += (float)g[j];
+        }
+    }
+#pragma unroll
+    for (int m = 0; m < MAXD; ++m) {
+        const int d = m * 256 + threadIdx.x;
+        if (d < band) line[1 + d] = acc[m];
+    }
+    left = re_wave_sum(left);
+    right = re_wave_sum(right);
+    if ((threadIdx.x & 63) == 0) {
+        tmp[threadIdx.x >> 6] = left;
+        tmp[4 + (threadIdx.x >> 6)] = right;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        line[0] = tmp[0] + tmp[1] + tmp[2] + tmp[3];
+        line[2 * R] = tmp[4] + tmp[5] + tmp[6] + tmp[7];
+    }
+    __syncthreads();
+    rb_line_to_buckets<256>(line, a.map, 2 * R + 1, a.buckets, static_cast<float*>(a.out) + (h * gridDim.x + blockIdx.x) * a.buckets, tmp);
+}
+
+template <class T>
+void rb_launch(bool bwd, const rb_args& a, bool vec, dim3 grid, hipStream_t st) {
+    constexpr int V = re_type<T>::VEC;
+    if (bwd) {
+        if (vec) hipLaunchKernelGGL((rb_bwd_k<T, V>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rb_bwd_k<T, 1>), grid, dim3(256), 0, st, a);
+    } else {
+        if (vec) hipLaunchKernelGGL((rb_fwd_k<T, V>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rb_fwd_k<T, 1>), grid, dim3(256), 0, st, a);
+    }
+}
+int rb_dispatch(bool bwd, const rb_args& a, int32_t dtype, const void* big, hipStream_t st) {
+    const bool vec = a.Sk % (16 / (int64_t)re_dtype_size(dtype)) == 0 && (reinterpret_cast<uintptr_t>(big) & 15) == 0;
+    const dim3 grid((unsigned)re_cdiv(a.Sq, RB_ROWS), (unsigned)a.H);
+    if (dtype == RE_F32) rb_launch<float>(bwd, a, vec, grid, st);
+    else if (dtype == RE_BF16) rb_launch<re_bf16>(bwd, a, vec, grid, st);
+    else rb_launch<re_f16>(bwd, a, vec, grid, st);
+    return 0;
+}
+bool rb_shape_ok(int64_t H, int64_t Sq, int64_t Sk) { return H >= 0 && Sq >= 0 && Sk >= 0 && H <= 65535 && Sq <= (1ll << 27) && Sk <= (1ll << 30); }
+int64_t rb_clip(int64_t offset) { return offset < -(1ll << 40) ? -(1ll << 40) : offset > (1ll << 40) ? (1ll << 40) : offset; }
+
+}  // namespace
+
+extern "C" int re_relative_bias_fwd(const void* table, const int32_t* bucket_map, int64_t buckets, int64_t max_distance, int64_t H, int64_t Sq,
+                                    int64_t Sk, int64_t offset, int32_t dtype, void* bias, re_stream_t stream) {
+    if (!re_dtype_size(dtype) || !rb_shape_ok(H, Sq, Sk) || buckets < 1 || max_distance < 1) return RE_EINVAL;
+    if (!rb_sizes_ok(max_distance, buckets)) return RE_EUNSUPPORTED;
+    if (H * Sq == 0 || Sk == 0) return RE_OK;
+    if (!table || !bucket_map || !bias) return RE_EINVAL;
+    re_clear_error();
+    const rb_args a{table, bias, bucket_map, H, Sq, Sk, rb_clip(offset), (int32_t)max_distance, (int32_t)buckets};
+    rb_dispatch(false, a, dtype, bias, (hipStream_t)stream);
+    return re_launch_status();
+}
+
+extern "C" size_t re_relative_bias_bwd_workspace_bytes(int64_t H, int64_t Sq, int64_t buckets) {
+    if (H < 1 || Sq < 1 || buckets < 1 || buckets > RB_MAX_BUCKETS) return 0;
+    return (size_t)H * (size_t)re_cdiv(Sq, RB_ROWS) * (size_t)buckets * sizeof(float);
+}
+
+extern "C" int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t buckets, int64_t max_distance, int64_t H, int64_t Sq,
+                                    int64_t Sk, int64_t offset, int32_t dtype, void* dtable, int32_t table_dtype, void* ws, size_t ws_bytes,
+                                    re_stream_t stream) {
+    if (!re_dtype_size(dtype) || !re_dtype_size(table_dtype) || !rb_shape_ok(H, Sq, Sk) || buckets < 1 || max_distance < 1) return RE_EINVAL;
+    if (!rb_sizes_ok(max_distance, buckets)) return RE_EUNSUPPORTED;
+    if (H == 0) return RE_OK;
+    const bool any = Sq > 0 && Sk > 0;
+    if (!dtable || (any && (!dbias || !bucket_map))) return RE_EINVAL;
+    if (any && (!ws || ws_bytes < re_relative_bias_bwd_workspace_bytes(H, Sq, buckets))) return RE_EWORKSPACE;
+    re_clear_error();
+    hipStream_t st = (hipStream_t)stream;
+    if (any) {
+        const rb_args a{dbias, ws, bucket_map, H, Sq, Sk, rb_clip(offset), (int32_t)max_distance, (int32_t)buckets};
+        rb_dispatch(true, a, dtype, dbias, st);
+    }
+    hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)H), dim3(256), 0, st, (const float*)ws, (int64_t)1, H, any ? re_cdiv(Sq, RB_ROWS) : 0,
+                       (int)buckets, dtable, table_dtype);
+    return re_launch_status();
+}

@@ -130,6 +130,12 @@ SIGNATURES = {
     "re_scale_copy": (_i32, [_vp, _vp, _f32, _i64, _vp]),
     "re_adam_step_dev": (_i32, [_vp, _vp, _vp, _vp, _i64, _vp, _f64, _f64, _f64, _f64, _vp]),
     "re_adam_step": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _f64, _f64, _f64, _f64, _f64, _vp]),
+    "re_layer_norm_fwd": (_i32, [_vp, _vp, _vp, _vp, _i64, _i64, _f32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "re_layer_norm_bwd_workspace_bytes": (_sz, [_i64, _i64]),
+    "re_layer_norm_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "re_relative_bias_fwd": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _vp]),
+    "re_relative_bias_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
+    "re_relative_bias_bwd": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _sz, _vp]),
 }
 
 _LIB = None

@@ -1521,3 +1521,159 @@ def colsum(x, out=None):
     ws = _ws(L.re_mlp_workspace_bytes(N), x.device)
     lib.check(L.re_colsum(_p(x), M, N, _p(out), _p(ws), ws.numel(), _stream()), "re_colsum")
     return out
+
+
+# ------------------------------------------------------------------------------------------------ transformer block: norm, position bias, attention
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}          # RE_F32 / RE_BF16 / RE_F16
+
+
+def _req_any(t, name, device=None, dtype=None, contiguous=True):
+    """`_req` for the operators that take fp32, bf16 and fp16: -> the tensor's RE_* code."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError(f"recengine: `{name}` must be a tensor on a HIP device (no CPU fallback exists)")
+    code = DTYPES.get(t.dtype)
+    if code is None or (dtype is not None and t.dtype != dtype):
+        raise TypeError(f"recengine: `{name}` must be {dtype or 'float32, bfloat16 or float16'}, got {t.dtype}")
+    if device is not None and t.device != device:
+        raise ValueError(f"recengine: `{name}` must be on {device}, got {t.device}")
+    if contiguous and not t.is_contiguous():
+        raise ValueError(f"recengine: `{name}` must be contiguous")
+    return code
+
+
+def _a(t):
+    return None if t is None else _note(t)
+
+
+def _call(device, fn, what, *args):
+    """fn(*args, stream) on the current stream of the tensors' device, whichever device is current."""
+    if device.index == torch.cuda.current_device():
+        lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+    else:
+        with torch.cuda.device(device):
+            lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+
+
+def _norm_params(x, weight, bias):
+    D = x.shape[-1] if x.dim() else 0
+    if D < 1:
+        raise ValueError("recengine: layer norm needs a last dimension of at least 1")
+    wtype = None
+    for t, nme in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        code = _req_any(t, nme, x.device)
+        if t.shape != (D,):
+            raise ValueError(f"recengine: `{nme}` must be [{D}], got {tuple(t.shape)}")
+        if wtype is not None and code != wtype:
+            raise TypeError("recengine: `weight` and `bias` must have one type")
+        wtype = code
+    return D, 0 if wtype is None else wtype
+
+
+def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """Layer norm over the last dimension of s = x (+ residual) (re_layer_norm_fwd): fp32, bf16 or fp16, contiguous; weight / bias [D] of
+    x's type or another of the three.  -> (y, s, mean, rstd): s is x itself without a residual, mean / rstd fp32, one for each row."""
+    code = _req_any(x, "x")
+    D, wtype = _norm_params(x, weight, bias)
+    y = torch.empty_like(x)
+    s = x
+    if residual is not None:
+        _req_any(residual, "residual", x.device, x.dtype)
+        if residual.shape != x.shape:
+            raise ValueError("recengine: `residual` must have x's shape")
+        s = torch.empty_like(x)
+    rows = x.numel() // D
+    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
+    mean, rstd = stats[0], stats[1]
+    _call(x.device, lib.load().re_layer_norm_fwd, "re_layer_norm_fwd", _a(x), _a(residual), _a(weight), _a(bias), rows, D, float(eps), code, wtype,
+          _a(y), _a(s) if residual is not None else None, _a(mean), _a(rstd))
+    return y, s, mean, rstd
+
+
+def layer_norm_bwd(dy, s, weight, mean, rstd, dsum=None, weight_grads=True):
+    """Backward of layer_norm_fwd (re_layer_norm_bwd): s, mean, rstd as it returned them, dsum the gradient that reaches s itself (a residual
+    stream that goes on).  -> (ds, dweight, dbias): ds is the gradient of x and of the residual; weight_grads=False: the last two are None."""
+    code = _req_any(s, "s")
+    _req_any(dy, "dy", s.device, s.dtype)
+    D, wtype = _norm_params(s, weight, None)
+    rows = s.numel() // D
+    if dy.shape != s.shape:
+        raise ValueError("recengine: `dy` must have s's shape")
+    for t, nme in ((mean, "mean"), (rstd, "rstd")):
+        _req_any(t, nme, s.device, torch.float32)
+        if t.numel() != rows:
+            raise ValueError(f"recengine: `{nme}` must hold one value for each row")
+    if dsum is not None:
+        _req_any(dsum, "dsum", s.device, s.dtype)
+        if dsum.shape != s.shape:
+            raise ValueError("recengine: `dsum` must have s's shape")
+    ds = torch.empty_like(s)
+    L = lib.load()
+    dw = db = ws = None
+    if weight_grads:
+        grads = torch.empty((2, D), dtype=torch.float32 if weight is None else weight.dtype, device=s.device)
+        dw, db = grads[0], grads[1]
+        ws = _ws(L.re_layer_norm_bwd_workspace_bytes(rows, D), s.device)
+    _call(s.device, L.re_layer_norm_bwd, "re_layer_norm_bwd", _a(dy), _a(s), _a(weight), _a(mean), _a(rstd), _a(dsum), rows, D, code, wtype, _a(ds),
+          _a(dw), _a(db), _a(ws), 0 if ws is None else ws.numel())
+    return ds, dw, db
+
+
+def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
+    """The bucket of every clipped distance key - query, [2 max_distance + 1] int32 (the operators' `bucket_map`): half of a side's buckets hold one
+    distance each, the others grow on a logarithmic scale up to max_distance, where the last begins; bidirectional: the upper half of the
+    buckets is for keys behind the query, otherwise those all share bucket 0.  The borders are found in whole numbers:
+    bucket exact + m begins at the least n with (n / exact)^steps >= (max_distance / exact)^m."""
+    side = num_buckets // 2 if bidirectional else num_buckets
+    exact = side // 2
+    if exact < 1 or num_buckets > 256 or not exact < max_distance <= 1024:
+        raise ValueError("recengine: relative buckets need 2 (bidirectional: 4) to 256 buckets and exact < max_distance <= 1024")
+    steps = side - exact
+    of = []
+    m = 0
+    for n in range(max_distance + 1):
+        while m + 1 < steps and n > exact and n ** steps >= max_distance ** (m + 1) * exact ** (steps - m - 1):
+            m += 1
+        of.append(n if n < exact else exact + m)
+    behind = [side + b for b in of[1:]] if bidirectional else [0] * max_distance
+    return torch.tensor(of[:0:-1] + [of[0]] + behind, dtype=torch.int32, device=device)
+
+
+def _req_map(bucket_map, device):
+    _req(bucket_map, torch.int32, "bucket_map")
+    n = bucket_map.numel()
+    if bucket_map.dim() != 1 or n % 2 == 0 or not 3 <= n <= 2049 or bucket_map.device != device:
+        raise ValueError("recengine: `bucket_map` must be [2 max_distance + 1] with max_distance 1 .. 1024, on the tensors' device")
+    return n // 2
+
+
+def relative_bias_fwd(table, bucket_map, queries, keys, offset=None):
+    """bias[h, i, j] = table[bucket_map[clip(j - (i + offset))], h], [H, queries, keys] in the table's type (re_relative_bias_fwd).  table:
+    [buckets, H]; offset: the first query's position among the keys, by default keys - queries (the queries are the last rows)."""
+    code = _req_any(table, "table")
+    if table.dim() != 2 or not 1 <= table.shape[0] <= 256:
+        raise ValueError("recengine: `table` must be [buckets, heads] with 1 .. 256 buckets")
+    far = _req_map(bucket_map, table.device)
+    H = table.shape[1]
+    bias = torch.empty((H, int(queries), int(keys)), dtype=table.dtype, device=table.device)
+    _call(table.device, lib.load().re_relative_bias_fwd, "re_relative_bias_fwd", _a(table), _a(bucket_map), table.shape[0], far, H, int(queries), int(keys),
+          int(keys) - int(queries) if offset is None else int(offset), code, _a(bias))
+    return bias
+
+
+def relative_bias_bwd(dbias, bucket_map, num_buckets, offset=None, dtype=None):
+    """dtable [num_buckets, H]: the sums of dbias [H, queries, keys] over the pairs of each bucket (re_relative_bias_bwd), in `dtype` (default:
+    dbias's type)."""
+    code = _req_any(dbias, "dbias")
+    dtype = dbias.dtype if dtype is None else dtype
+    if dbias.dim() != 3 or not 1 <= int(num_buckets) <= 256 or dtype not in DTYPES:
+        raise ValueError("recengine: `dbias` must be [heads, queries, keys], the table at most 256 buckets of float32, bfloat16 or float16")
+    far = _req_map(bucket_map, dbias.device)
+    H, queries, keys = dbias.shape
+    L = lib.load()
+    dtable = torch.empty((int(num_buckets), H), dtype=dtype, device=dbias.device)
+    ws = _ws(L.re_relative_bias_bwd_workspace_bytes(H, queries, int(num_buckets)), dbias.device)
+    _call(dbias.device, L.re_relative_bias_bwd, "re_relative_bias_bwd", _a(dbias), _a(bucket_map), int(num_buckets), far, H, queries, keys,
+          keys - queries if offset is None else int(offset), code, _a(dtable), DTYPES[dtype], _a(ws), ws.numel())
+    return dtable
