@@ -749,6 +749,44 @@ int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t b
                          int64_t Sk, int64_t offset, int32_t dtype, void* dtable, int32_t table_dtype, void* ws, size_t ws_bytes,
                          re_stream_t stream);
 
+/* Attention:  out = softmax over the keys a row may see of (scale q k^T + bias + mask), times v;  stats = each row's largest score and the log
+ * of its sum of exp(score - largest): their sum is the log of the softmax's denominator, and apart they serve rows of any magnitude.
+ * q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], Hkv a divisor of Hq (query head h reads key head h / (Hq / Hkv)), any batch / head / row
+ * strides (in elements, 0 for a broadcast one), D adjacent elements in a row, 1 <= D <= 128.
+ * The keys that query i of sequence b may see: j < key_lengths[b] (DEVICE int64 [B], optional; values outside [0, Sk] are clipped), with
+ * `causal` also j <= o + i, and the mask's; o = q_offsets[b] (DEVICE int64 [B]) or, when NULL, q_offset: the position of query 0 among
+ * the keys.  mask (optional) has four strides (batch, query head, query, key; 0 where it is broadcast) and is
+ * mask_kind 1: one byte a place, 0 = shut;  2 / 3 / 4: added to the score, fp32 / bf16 / fp16, -inf = shut.
+ * bias = table[bucket_map[clip(j - (o + i), -R, R) + R], h] (re_relative_bias_fwd; table [buckets, Hq], NULL: none; R = max_distance).
+ * A key that is shut for a row has no part in it, whatever k and v hold there.  A row that sees no key: out 0, stats (-inf, 0), no
+ * gradients.
+ * The rows of k and v behind key_lengths[b] are not read.  scale > 0. */
+typedef struct re_attention {
+    const void *q, *k, *v;
+    int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, row */
+    int64_t B, Hq, Hkv, Sq, Sk, D;
+    const void* mask;
+    int64_t mask_stride[4];
+    const int64_t *key_lengths, *q_offsets;
+    int64_t q_offset;
+    const void* table;
+    const int32_t* bucket_map;
+    int64_t buckets, max_distance;
+    float scale;
+    int32_t dtype, causal, mask_kind, table_dtype, reserved;
+} re_attention;
+
+/* out: strides `out_stride` (batch, head, row), stats [2, B, Hq, Sq] contiguous.  Few rows against many keys (one new token per sequence) are
+ * split over the keys and joined: the workspace holds the parts (0 bytes where nothing is split). */
+size_t re_attention_fwd_workspace_bytes(const re_attention* a);
+int re_attention_fwd(const re_attention* a, void* out, const int64_t* out_stride, float* stats, void* ws, size_t ws_bytes, re_stream_t stream);
+/* Its backward: q, k, v, ... as in the forward call, its out and stats, and dout (strides `dout_stride`).  dq, dk, dv: the inputs' type, any
+ * strides, every row written (rows of keys that no row sees: 0).  dtable [buckets, Hq] of type table_dtype, or NULL. */
+size_t re_attention_bwd_workspace_bytes(const re_attention* a);
+int re_attention_bwd(const re_attention* a, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
+                     const int64_t* dout_stride, void* dq, const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,
+                     const int64_t* dv_stride, void* dtable, void* ws, size_t ws_bytes, re_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,66 @@
+// Attention, backward: the entry point, its workspace and the rule that chooses the kernels' shapes (the kernels: attn_bwd.inc).
+#include "attn_bwd.h"
+
+namespace attn {
+
+static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_table) {
+    bwd_plan p{};
+    p.vec = vec;
+    p.mod = a.table || a.mkind >= 2;
+    p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
+    p.wq = a.Sq <= 64 ? 2 : 4;
+    p.wk = a.Sk <= 64 ? 2 : 4;
+    p.qtiles = re_cdiv(a.Sq, 32 * p.wq);
+    p.ktiles = re_cdiv(a.Sk, 32 * p.wk);
+    const int rows = dtype == RE_F32 ? 32 : 64;
+    const int ch = p.dp * (int)re_dtype_size(dtype) / 16;
+    const int chp = dtype == RE_F32 ? ch + 1 : ch <= 4 ? 4 : ch <= 8 ? 8 : 16;
+    const size_t tiles = (size_t)4 * rows * chp * 16, n_line = 2 * a.R + 1;
+    p.lds_q = tiles + (a.table ? n_line * sizeof(float) : 0) + (want_table ? p.wq * (n_line + 32 * 33) * sizeof(float) : 0);
+    p.lds_k = tiles + 6 * rows * sizeof(float) + (a.table ? n_line * sizeof(float) : 0);
+    return p;
+}
+static size_t delta_bytes(const args& a) { return re_align((size_t)a.B * a.Hq * a.Sq * sizeof(float)); }
+static size_t part_bytes(const args& a, const bwd_plan& p) { return (size_t)a.B * a.Hq * p.qtiles * a.buckets * sizeof(float); }
+
+}  // namespace attn
+
+extern "C" size_t re_attention_bwd_workspace_bytes(const re_attention* d) {
+    attn::args a;
+    if (attn_args(d, a) != RE_OK || attn_empty(a)) return 0;
+    return attn::delta_bytes(a) + (a.table ? attn::part_bytes(a, attn::make_bwd_plan(a, d->dtype, false, true)) : 0);
+}
+
+extern "C" int re_attention_bwd(const re_attention* d, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
+                                const int64_t* dout_stride, void* dq, const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,
+                                const int64_t* dv_stride, void* dtable, void* ws, size_t ws_bytes, re_stream_t stream) {
+    attn::args a;
+    const int rc = attn_args(d, a);
+    if (rc != RE_OK) return rc;
+    if (!out_stride || !dout_stride || !dq_stride || !dk_stride || !dv_stride || (dtable && !a.table)) return RE_EINVAL;
+    if (attn_empty(a)) return a.B && a.Hq && a.Sk ? RE_EUNSUPPORTED : RE_OK;      // (no query, but gradients of keys to write: the caller's zeros)
+    if (!a.q || !out || !stats || !dout || !dq || (a.Sk > 0 && (!a.k || !a.v || !dk || !dv))) return RE_EINVAL;
+    const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}, {dout, dout_stride}, {dq, dq_stride},
+                                                {dk, dk_stride}, {dv, dv_stride}});
+    const attn::bwd_plan p = attn::make_bwd_plan(a, d->dtype, vec, dtable != nullptr);
+    if ((int64_t)a.B * a.Hq * p.qtiles >= (1ll << 23) || (int64_t)a.B * a.Hkv * p.ktiles >= (1ll << 23)) return RE_EUNSUPPORTED;
+    const size_t need = attn::delta_bytes(a) + (dtable ? attn::part_bytes(a, p) : 0);
+    if (!ws || ws_bytes < need) return RE_EWORKSPACE;
+    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, dtable ? (float*)((char*)ws + attn::delta_bytes(a)) : nullptr};
+    for (int x = 0; x < 3; ++x) {
+        io.os[x] = out_stride[x];
+        io.dos[x] = dout_stride[x];
+        io.dqs[x] = dq_stride[x];
+        io.dks[x] = dk_stride[x];
+        io.dvs[x] = dv_stride[x];
+    }
+    re_clear_error();
+    hipStream_t st = (hipStream_t)stream;
+    const int r = d->dtype == RE_F32 ? attn::bwd_launch<float>(a, io, p, st) : d->dtype == RE_BF16 ? attn::bwd_launch<re_bf16>(a, io, p, st)
+                                                                                              : attn::bwd_launch<re_f16>(a, io, p, st);
+    if (r != RE_OK) return r;
+    if (dtable)
+        hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)a.Hq), dim3(256), 0, st, io.part, (int64_t)a.B, (int64_t)a.Hq, p.qtiles, a.buckets, dtable,
+                           a.tdtype);
+    return re_launch_status();
+}

@@ -1,0 +1,342 @@
+// What the attention kernels share: arguments, tiles in LDS, matrix-instruction fragments, scores and masks.
+//
+// Every product is made with the 32 x 32 matrix instructions (16-bit types: 32x32x16, fp32: 32x32x2), whose result has, in lane l, column l % 32
+// and rows 8 (r / 4) + 4 (l / 32) + r % 4 for its registers r = 0 .. 15.  The kernels are laid out so that the index a softmax runs over is
+// the ROW of such a result: a lane then owns whole columns (one query, or one key), its maximum and sum need one exchange with the other
+// half of the wave, and -- since the order of a contraction is free -- the result's registers are, converted, the right-hand operand of
+// the next product as they stand:  registers 8 s .. 8 s + 7 are the contraction indexes {16 s + 4 half + 0 .. 3, 16 s + 8 + 4 half + 0 .. 3},
+// and the left-hand operand is fetched for those same indexes (ds_read_b64_tr_b16: four consecutive rows of a row-major tile, one column
+// per lane).  Probabilities and score gradients never leave the registers.
+#pragma once
+#include "relbias.h"
+
+#define ATTN_MAX_D 128
+#define ATTN_LOG2E 1.44269504088896340736f
+#define ATTN_LN2 0.69314718055994530942f
+
+#ifdef __HIPCC__
+namespace attn {
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef re_bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef re_f16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+
+#define ATTN_INF __builtin_inff()
+
+struct args {
+    const void *q, *k, *v;
+    int64_t qs[3], ks[3], vs[3];       // strides in elements: batch, head, row (adjacent inside a row)
+    int32_t B, Hq, Hkv, Sq, Sk, D, group;
+    float scale;
+    int32_t causal, mkind;             // mkind: 0 none, 1 truth values, 2 / 3 / 4 additive fp32 / bf16 / fp16
+    const void* mask;
+    int64_t ms[4];                     // batch, head, query, key
+    const int64_t *lens, *offs;
+    int64_t off;
+    const void* table;
+    const int32_t* map;
+    int32_t tdtype, R, buckets;
+};
+
+// ---------------------------------------------------------------------------------------------------------- matrix instructions
+// A fragment is 16 bytes a lane: KS contraction indexes of a 32-wide operand, the lane's own KS / 2 of them at 16 bytes * half.
+template <class T>
+struct mm;
+template <>
+struct mm<re_bf16> {
+    typedef bf16x8 frag;
+    static constexpr int KS = 16;
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct mm<re_f16> {
+    typedef f16x8 frag;
+    static constexpr int KS = 16;
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct mm<float> {
+    typedef f32x4 frag;
+    static constexpr int KS = 8;
+    static __device__ __forceinline__ f32x16 mul(frag a, frag b, f32x16 c) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[i], b[i], c, 0, 0, 0);
+        return c;
+    }
+};
+
+// ---------------------------------------------------------------------------------------------------------- tiles
+// A tile is ROWS rows of a tensor in LDS, row-major in 16-byte chunks.  16-bit types: the chunk of a row is moved by an exclusive or with
+// a value of the row such that both kinds of reads -- 16 rows at one chunk (row fragments) and 4 rows at 4 chunks (transposed
+// fragments) -- fall on distinct banks; fp32: rows are padded by one chunk (its column reads meet two-fold conflicts).
+template <class T, int DP>
+struct tile {
+    static constexpr int EPC = 16 / (int)sizeof(T);                  // elements of a chunk
+    static constexpr int CH = DP / EPC;                              // chunks of a row
+    static constexpr int CHP = sizeof(T) == 4 ? CH + 1 : CH <= 4 ? 4 : CH <= 8 ? 8 : 16;      // ... as laid out
+    static constexpr int ROW = CHP * EPC;                            // elements between rows
+    static __device__ __forceinline__ int swz(int row) {
+        if constexpr (sizeof(T) == 4) return 0;
+        else if constexpr (CHP == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+        else if constexpr (CHP == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+        else return (row >> 2) & 3;
+    }
+    static __device__ __forceinline__ int at(int row, int chunk) { return row * ROW + ((chunk ^ swz(row)) * EPC); }
+    static constexpr size_t bytes(int rows) { return (size_t)rows * CHP * 16; }
+};
+
+// ROWS x DP elements of a tensor, through the registers of THREADS lanes: load() issues, store() writes to LDS.  Rows from `rows` on and
+// columns from D on are zero and not read.  VEC: every row starts on 16 bytes and D is whole chunks; otherwise element by element.
+template <class T, int DP, int ROWS, int THREADS, bool VEC>
+struct stage {
+    typedef tile<T, DP> tl;
+    static constexpr int N = ROWS * tl::CH / THREADS;
+    static_assert(ROWS * tl::CH % THREADS == 0, "whole chunks for each lane");
+    uint4 r[N];
+    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int D) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = n * THREADS + (int)threadIdx.x, row = c / tl::CH, e = (c % tl::CH) * tl::EPC;
+            r[n] = make_uint4(0, 0, 0, 0);
+            if constexpr (VEC) {
+                if (row < rows && e < D) r[n] = *reinterpret_cast<const uint4*>(base + row * stride + e);
+            } else {
+                union { uint4 u; T t[tl::EPC]; } x;
+                x.u = r[n];
+#pragma unroll
+                for (int i = 0; i < tl::EPC; ++i)
+                    if (row < rows && e + i < D) x.t[i] = base[row * stride + e + i];
+                r[n] = x.u;
+            }
+        }
+    }
+    __device__ __forceinline__ void store(T* lds) const {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int c = n * THREADS + (int)threadIdx.x;
+            *reinterpret_cast<uint4*>(lds + tl::at(c / tl::CH, c % tl::CH)) = r[n];
+        }
+    }
+};
+
+// a row's own fragments straight from memory (the operand that a wave keeps): 16 bytes at KS * step + KS / 2 * half
+template <class T, int DP, bool VEC>
+__device__ __forceinline__ void load_row_frags(const T* row, bool live, int D, int half, typename mm<T>::frag* f) {
+    typedef typename mm<T>::frag frag;
+    constexpr int EPC = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int s = 0; s < DP / mm<T>::KS; ++s) {
+        const int e = s * mm<T>::KS + half * EPC;
+        union { frag f; uint4 u; T t[EPC]; } x;
+        x.u = make_uint4(0, 0, 0, 0);
+        if constexpr (VEC) {
+            if (live && e < D) x.u = *reinterpret_cast<const uint4*>(row + e);
+        } else {
+#pragma unroll
+            for (int i = 0; i < EPC; ++i)
+                if (live && e + i < D) x.t[i] = row[e + i];
+        }
+        f[s] = x.f;
+    }
+}
+
+// left-hand operand, rows of a tile: lane l holds row row0 + l % 32
+template <class T, int DP>
+__device__ __forceinline__ typename mm<T>::frag row_frag(const T* lds, int row, int step, int half) {
+    typedef tile<T, DP> tl;
+    return *reinterpret_cast<const typename mm<T>::frag*>(lds + tl::at(row, 2 * step + half));
+}
+
+// left-hand operand, COLUMNS of a tile: lane l holds column col0 + l % 32; the contraction runs over the rows that registers
+// PR s .. PR s + PR - 1 of a 32 x 32 result stand for (PR = 8, fp32: 4); row0: the block's first row
+template <class T, int DP>
+__device__ __forceinline__ typename mm<T>::frag col_frag(const T* lds, int row0, int s, int col0, int lane) {
+    typedef tile<T, DP> tl;
+    const int half = lane >> 5;
+    if constexpr (sizeof(T) == 4) {
+        f32x4 f;
+        const int c = col0 + (lane & 31);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[i] = lds[(row0 + 8 * s + 4 * half + i) * tl::ROW + c];
+        return f;
+    } else {
+        // a group of 16 lanes reads 4 rows x 16 columns, 4 elements a lane, and gets 4 rows of one column a lane
+        const int i = lane & 15;
+        const int chunk = (col0 >> 3) + ((lane >> 4) & 1) * 2 + ((i >> 1) & 1);
+        union { s16x4 h[2]; typename mm<T>::frag f; } x;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+            const int row = row0 + 16 * s + 8 * p + 4 * half + (i >> 2);
+            const T* at = lds + tl::at(row, chunk) + (i & 1) * 4;
+            x.h[p] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
+        }
+        return x.f;
+    }
+}
+
+// registers PR s .. of a result as the right-hand operand of the next product (16-bit types: one rounding, to nearest)
+template <class T>
+__device__ __forceinline__ typename mm<T>::frag reg_frag(const f32x16& x, int s) {
+    typename mm<T>::frag f;
+    constexpr int PR = sizeof(T) == 4 ? 4 : 8;
+#pragma unroll
+    for (int i = 0; i < PR; ++i) f[i] = (T)x[PR * s + i];
+    return f;
+}
+template <class T>
+constexpr int frags_of_block() { return sizeof(T) == 4 ? 4 : 2; }
+
+__device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
+__device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
+
+// ---------------------------------------------------------------------------------------------------------- lengths, masks, bias
+__device__ __forceinline__ int seq_len(const args& a, int b) {
+    if (!a.lens) return a.Sk;
+    const int64_t n = a.lens[b];
+    return n < 0 ? 0 : n > a.Sk ? a.Sk : (int)n;
+}
+// the position of query 0 among the keys; clipped where nothing changes any more (keys and queries are below 2^30)
+__device__ __forceinline__ int seq_off(const args& a, int b) {
+    const int64_t o = a.offs ? a.offs[b] : a.off;
+    return o < -(1 << 30) ? -(1 << 30) : o > (1 << 30) - 1 ? (1 << 30) - 1 : (int)o;
+}
+// additive value of the mask; a truth value that is false and -inf shut the place
+__device__ __forceinline__ float mask_add(const args& a, int64_t at) {
+    if (a.mkind == 1) return static_cast<const uint8_t*>(a.mask)[at] ? 0.f : -ATTN_INF;
+    return re_load_as_float(a.mask, at, a.mkind - 2);
+}
+__device__ __forceinline__ int clip_distance(int d, int R) { return d < -R ? -R : d > R ? R : d; }
+
+// the bias of `heads` heads from h0 on, [heads][2 R + 1] in LDS
+template <int THREADS>
+__device__ __forceinline__ void load_lines(const args& a, int h0, int heads, float* line) {
+    const int n = 2 * a.R + 1;
+    for (int x = threadIdx.x; x < heads * n; x += THREADS)
+        line[x] = rb_entry(a.table, a.tdtype, a.map, x % n, a.buckets, a.Hq, h0 + x / n);
+}
+
+// Does the mask depend on the key alone (within a sequence)?  Then a tile's part of it is one bit a key.
+__device__ __forceinline__ bool mask_by_key(const args& a) { return a.mkind == 1 && a.ms[1] == 0 && a.ms[2] == 0; }
+
+// One score, outside the matrix path: raw = q . k; -> the score, vis = false where the row may not see the key
+__device__ __forceinline__ float score_of(const args& a, float raw, int b, int h, int i, int j, int len, int off, const float* line, bool& vis,
+                                          bool no_bias = false) {
+    vis = j < len && !(a.causal && j > off + i);
+    float s = raw * a.scale;
+    if (!vis) return -ATTN_INF;
+    if (a.table && !no_bias) s += line[clip_distance(j - (off + i), a.R) + a.R];
+    if (a.mkind) {
+        const float m = mask_add(a, b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + j * a.ms[3]);
+        if (m == -ATTN_INF) vis = false;
+        s += m;
+    }
+    return vis ? s : -ATTN_INF;
+}
+template <class T>
+__device__ __forceinline__ float dot_rows(const T* x, const T* y, int D) {
+    float s = 0.f;
+    for (int d = 0; d < D; ++d) s += (float)x[d] * (float)y[d];
+    return s;
+}
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+__device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) < ATTN_INF); }
+
+// A 32 x 32 block of raw products -> scores (MOD: bias or additive mask) or the products as they are (otherwise), shut places -inf.  Scores stay
+// in natural units: a mask of the type's lowest value would overflow as a multiple of log2 e, and a row that holds nothing else has
+// to come out even.
+// The lane's column is query (i, h) and rows are keys j0 + row_of (BY_KEY = false), or the column is key j and rows are queries (true).
+// bits: the tile's keys that are there (length and by-key mask), bit 0 = key j0; only with keys as rows.
+template <bool MOD>
+__device__ __forceinline__ void apply_keys(const args& a, f32x16& s, int b, int h, int i, int j0, int half, int off, uint32_t bits, bool diag,
+                                           const float* line) {
+    if constexpr (MOD) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= a.scale;
+        if (a.table) {
+            const int d0 = j0 - (off + i);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] += line[clip_distance(d0 + row_of(r, half), a.R) + a.R];
+        }
+    }
+    if (a.mkind && !mask_by_key(a)) {
+        const int64_t at = b * a.ms[0] + h * a.ms[1] + (int64_t)i * a.ms[2] + (int64_t)j0 * a.ms[3];
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int row = row_of(r, half);
+            if (bits >> row & 1) {                      // (a key that is there: its mask may be read)
+                const float m = mask_add(a, at + row * a.ms[3]);
+                s[r] = m == -ATTN_INF ? -ATTN_INF : MOD ? s[r] + m : s[r];
+            }
+        }
+    }
+    if (bits != 0xffffffffu) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = bits >> row_of(r, half) & 1 ? s[r] : -ATTN_INF;
+    }
+    if (diag) {
+        const int last = off + i - j0;                  // the last key that the query sees, within the block
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = row_of(r, half) > last ? -ATTN_INF : s[r];
+    }
+}
+// exp(s - m) of a block's score; mu: m in natural units (MOD) or m * scale * log2 e of the products' units
+template <bool MOD>
+__device__ __forceinline__ float exp_of(float s, float mu, float c1) {
+    if constexpr (MOD) return exp2f((s - mu) * ATTN_LOG2E);
+    else return exp2f(s * c1 - mu);
+}
+// bits of keys j0 .. j0 + 63 that are there; every lane of a wave calls it
+__device__ __forceinline__ uint64_t key_bits(const args& a, int b, int j0, int len, bool by_key, int lane) {
+    const int j = j0 + lane;
+    bool there = j < len;
+    if (there && by_key) there = static_cast<const uint8_t*>(a.mask)[b * a.ms[0] + j * a.ms[3]] != 0;
+    return __ballot(there);
+}
+
+}  // namespace attn
+
+// ---------------------------------------------------------------------------------------------------------- host
+#include <initializer_list>
+
+static inline int attn_args(const re_attention* d, attn::args& a) {
+    if (!d || !re_dtype_size(d->dtype)) return RE_EINVAL;
+    if (d->B < 0 || d->Hq < 0 || d->Hkv < 1 || d->Sq < 0 || d->Sk < 0 || d->D < 1 || d->Hq % d->Hkv) return RE_EINVAL;
+    if (d->D > ATTN_MAX_D || d->Sq > (1 << 30) - 1 || d->Sk > (1 << 30) - 1 || d->B > (1 << 24) || d->Hq > (1 << 16)) return RE_EUNSUPPORTED;
+    if (!(d->scale > 0.f) || d->scale > 1e30f) return RE_EINVAL;
+    if (d->mask ? d->mask_kind < 1 || d->mask_kind > 4 : d->mask_kind != 0) return RE_EINVAL;
+    if (d->table) {
+        if (!d->bucket_map || !re_dtype_size(d->table_dtype)) return RE_EINVAL;
+        if (!rb_sizes_ok(d->max_distance, d->buckets)) return RE_EUNSUPPORTED;
+    }
+    a = attn::args{d->q, d->k, d->v, {d->q_stride[0], d->q_stride[1], d->q_stride[2]}, {d->k_stride[0], d->k_stride[1], d->k_stride[2]},
+                   {d->v_stride[0], d->v_stride[1], d->v_stride[2]}, (int32_t)d->B, (int32_t)d->Hq, (int32_t)d->Hkv, (int32_t)d->Sq, (int32_t)d->Sk,
+                   (int32_t)d->D, (int32_t)(d->Hq / d->Hkv), d->scale, d->causal != 0, d->mask_kind, d->mask,
+                   {d->mask_stride[0], d->mask_stride[1], d->mask_stride[2], d->mask_stride[3]}, d->key_lengths, d->q_offsets, d->q_offset, d->table,
+                   d->bucket_map, d->table_dtype, d->table ? (int32_t)d->max_distance : 0, d->table ? (int32_t)d->buckets : 0};
+    return RE_OK;
+}
+static inline bool attn_empty(const attn::args& a) { return a.B == 0 || a.Hq == 0 || a.Sq == 0; }
+
+struct attn_tensor {
+    const void* p;
+    const int64_t* stride;
+};
+// every row of every tensor starts on 16 bytes, and is whole 16-byte chunks
+static inline bool attn_aligned(const attn::args& a, int32_t dtype, std::initializer_list<attn_tensor> ts) {
+    const int64_t epc = 16 / (int64_t)re_dtype_size(dtype);
+    if (a.D % epc) return false;
+    for (const attn_tensor& t : ts) {
+        if (reinterpret_cast<uintptr_t>(t.p) & 15) return false;
+        for (int x = 0; x < 3; ++x)
+            if (t.stride[x] % epc) return false;
+    }
+    return true;
+}
+#endif

@@ -1,0 +1,25 @@
+// The launch of attention's forward kernels, between the entry point (attn_fwd.hip) and the instances for each type (attn_fwd_*.hip).
+#pragma once
+#include "attn_common.h"
+
+namespace attn {
+
+struct fwd_out {
+    void* o;
+    int64_t os[3];                 // batch, head, row
+    float* stats;                  // [max, log sum][B][Hq][Sq]
+    float* part;                   // [splits][B][Hq][Sq][D], then [splits][B][Hq][Sq][2]; null: one split
+    int32_t splits, tiles, heads, pg, xcd;   // heads: workgroup heads per sequence; pg: query heads that share a workgroup's rows
+};
+
+struct fwd_plan {
+    int wq, wk, pg, tiles, heads, splits, bk;
+    bool mod, vec;
+    int dp;
+    size_t lds, part;     // bytes of LDS; of workspace
+};
+
+template <class T>
+int fwd_launch(const args& a, const fwd_out& f, const fwd_plan& p, hipStream_t st);
+
+}  // namespace attn

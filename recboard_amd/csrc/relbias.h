@@ -21,16 +21,20 @@ __device__ __forceinline__ float rb_entry(const void* table, int32_t dtype, cons
 template <int THREADS>
 __device__ __forceinline__ void rb_line_to_buckets(const float* line, const int32_t* __restrict__ map, int n, int buckets, float* out, float* tmp) {
     int p = 1;
-    while (p < buckets) p <<= 1;                       // (<= 256 = THREADS at least)
-    const int k = threadIdx.x & (p - 1), slice = threadIdx.x / p, slices = THREADS / p;
-    float acc = 0.f;
+    while (p < buckets && p < THREADS) p <<= 1;
+    const int slice = threadIdx.x / p, slices = THREADS / p;
     const int per = (n + slices - 1) / slices, from = slice * per, to = min(n, from + per);
-    for (int d = from; d < to; ++d) acc += map[d] == k ? line[d] : 0.f;
-    tmp[threadIdx.x] = acc;
-    __syncthreads();
-    if (slice == 0 && k < buckets) {
-        for (int s = 1; s < slices; ++s) acc += tmp[s * p + k];
-        out[k] = acc;
+    for (int k0 = 0; k0 < buckets; k0 += p) {
+        const int k = k0 + (threadIdx.x & (p - 1));
+        float acc = 0.f;
+        for (int d = from; d < to; ++d) acc += map[d] == k ? line[d] : 0.f;
+        __syncthreads();                               // (the last round's parts have been read)
+        tmp[threadIdx.x] = acc;
+        __syncthreads();
+        if (slice == 0 && k < buckets) {
+            for (int s = 1; s < slices; ++s) acc += tmp[s * p + (k - k0)];
+            out[k] = acc;
+        }
     }
 }
 

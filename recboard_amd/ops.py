@@ -1677,3 +1677,143 @@ def relative_bias_bwd(dbias, bucket_map, num_buckets, offset=None, dtype=None):
     _call(dbias.device, L.re_relative_bias_bwd, "re_relative_bias_bwd", _a(dbias), _a(bucket_map), int(num_buckets), far, H, queries, keys,
           keys - queries if offset is None else int(offset), code, _a(dtable), DTYPES[dtype], _a(ws), ws.numel())
     return dtable
+
+
+class _Attention(ctypes.Structure):          # re_attention (include/recengine.h)
+    _fields_ = [("q", ctypes.c_void_p), ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("q_stride", ctypes.c_int64 * 3), ("k_stride", ctypes.c_int64 * 3),
+                ("v_stride", ctypes.c_int64 * 3), ("B", ctypes.c_int64), ("Hq", ctypes.c_int64), ("Hkv", ctypes.c_int64), ("Sq", ctypes.c_int64),
+                ("Sk", ctypes.c_int64), ("D", ctypes.c_int64), ("mask", ctypes.c_void_p), ("mask_stride", ctypes.c_int64 * 4),
+                ("key_lengths", ctypes.c_void_p), ("q_offsets", ctypes.c_void_p), ("q_offset", ctypes.c_int64), ("table", ctypes.c_void_p),
+                ("bucket_map", ctypes.c_void_p), ("buckets", ctypes.c_int64), ("max_distance", ctypes.c_int64), ("scale", ctypes.c_float),
+                ("dtype", ctypes.c_int32), ("causal", ctypes.c_int32), ("mask_kind", ctypes.c_int32), ("table_dtype", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
+_STRIDE3 = ctypes.c_int64 * 3
+
+
+def _rows4(t, name, like=None):
+    """A [batch, head, row, D] operand with adjacent elements in a row: -> its RE_* code, its three strides."""
+    code = _req_any(t, name, *((like.device, like.dtype) if like is not None else ()), contiguous=False)
+    if t.dim() != 4:
+        raise ValueError(f"recengine: `{name}` must be [batch, heads, rows, D], got {tuple(t.shape)}")
+    st = t.stride()
+    if st[3] != 1 and t.shape[3] != 1:
+        raise ValueError(f"recengine: `{name}` must have adjacent elements in a row (stride 1 in the last dimension)")
+    return code, _STRIDE3(st[0], st[1], st[2])
+
+
+def _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_table, bucket_map):
+    d = _Attention()
+    d.dtype, d.q_stride = _rows4(q, "q")
+    d.k_stride, d.v_stride = _rows4(k, "k", q)[1], _rows4(v, "v", q)[1]
+    dev = q.device
+    B, Hq, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or v.shape != k.shape or Hkv < 1 or Hq % Hkv:
+        raise ValueError(f"recengine: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)} do not fit (k and v of one shape, key heads a divisor of "
+                         "query heads)")
+    if not 1 <= D <= 128:
+        raise ValueError(f"recengine: attention takes head sizes 1 .. 128, got {D}")
+    d.q, d.k, d.v = _a(q), _a(k), _a(v)
+    d.B, d.Hq, d.Hkv, d.Sq, d.Sk, d.D = B, Hq, Hkv, Sq, Sk, D
+    d.scale = D ** -0.5 if scale is None else float(scale)
+    if not 0.0 < d.scale < 1e30:
+        raise ValueError("recengine: `scale` must be positive")
+    d.causal = bool(causal)
+    if mask is not None:
+        if not isinstance(mask, torch.Tensor) or mask.device != dev:
+            raise ValueError("recengine: `mask` must be a tensor on q's device")
+        if mask.dtype == torch.bool:
+            d.mask_kind = 1
+        elif mask.dtype in DTYPES:
+            d.mask_kind = 2 + DTYPES[mask.dtype]
+        else:
+            raise TypeError(f"recengine: `mask` must be bool (True: may be seen) or floating (added), got {mask.dtype}")
+        try:
+            e = mask.expand(B, Hq, Sq, Sk)
+        except RuntimeError:
+            raise ValueError(f"recengine: `mask` {tuple(mask.shape)} does not broadcast to {(B, Hq, Sq, Sk)}") from None
+        d.mask_stride = (ctypes.c_int64 * 4)(*(s if n > 1 else 0 for s, n in zip(e.stride(), e.shape)))
+        if e.numel():
+            d.mask = _a(mask)
+        else:
+            d.mask_kind = 0
+    if key_lengths is not None:
+        _req(key_lengths, torch.int64, "key_lengths")
+        if key_lengths.shape != (B,) or key_lengths.device != dev:
+            raise ValueError("recengine: `key_lengths` must be [batch], on q's device")
+        d.key_lengths = _a(key_lengths)
+    if isinstance(q_offset, torch.Tensor):
+        _req(q_offset, torch.int64, "q_offset")
+        if q_offset.shape != (B,) or q_offset.device != dev:
+            raise ValueError("recengine: `q_offset` must be an int or [batch], on q's device")
+        d.q_offsets = _a(q_offset)
+    else:
+        d.q_offset = Sk - Sq if q_offset is None else int(q_offset)
+    if (rel_table is None) != (bucket_map is None):
+        raise ValueError("recengine: `rel_table` and `bucket_map` go together")
+    if rel_table is not None:
+        d.table_dtype = _req_any(rel_table, "rel_table", dev)
+        if rel_table.dim() != 2 or rel_table.shape[1] != Hq or not 1 <= rel_table.shape[0] <= 256:
+            raise ValueError(f"recengine: `rel_table` must be [buckets, {Hq}] with 1 .. 256 buckets")
+        d.max_distance = _req_map(bucket_map, dev)
+        d.buckets = rel_table.shape[0]
+        d.table, d.bucket_map = _a(rel_table), _a(bucket_map)
+    return d
+
+
+def _heads_of(B, S, H, D, like):
+    """An empty [B, H, S, D] whose memory is [B, S, H, D]: what the output projection (and a joint q / k / v projection) reads as rows."""
+    return torch.empty((B, S, H, D), dtype=like.dtype, device=like.device).transpose(1, 2)
+
+
+def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, rel_table=None, bucket_map=None):
+    """softmax(scale q k^T + bias + mask) v over the keys that a row may see (re_attention_fwd): q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], fp32,
+    bf16 or fp16, any strides but adjacent elements in a row, D <= 128; Hkv a divisor of Hq (shared key heads).
+
+        scale         1 / sqrt(D) by default
+        causal        query i sees keys j <= q_offset + i
+        mask          broadcasts to [B, Hq, Sq, Sk]: bool (True: may be seen) or floating (added to the scores; -inf shuts); takes no gradient
+        key_lengths   int64 [B]: the keys that a sequence has; rows behind are not read
+        q_offset      the position of query 0 among the keys: an int or int64 [B]; Sk - Sq by default (the queries are the last rows).  With
+                      key_lengths of a cache: key_lengths - Sq.
+        rel_table, bucket_map   the relative position bias (relative_bias_fwd), made inside: table [buckets, Hq]
+
+    -> (out [B, Hq, Sq, D] laid out as [B, Sq, Hq, D], stats [2, B, Hq, Sq] fp32: the largest score of a row and the log of its sum, which add
+    up to the log of the softmax's denominator).  A row that sees no key: out 0, stats -inf and 0."""
+    d = _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_table, bucket_map)
+    B, Hq, Sq, D = q.shape
+    out = _heads_of(B, Sq, Hq, D, q)
+    stats = torch.empty((2, B, Hq, Sq), dtype=torch.float32, device=q.device)
+    L = lib.load()
+    p = ctypes.addressof(d)
+    n = L.re_attention_fwd_workspace_bytes(p)
+    ws = _ws(n, q.device) if n else None
+    st = out.stride()
+    _call(q.device, L.re_attention_fwd, "re_attention_fwd", p, _a(out), _STRIDE3(st[0], st[1], st[2]), _a(stats), _a(ws), n)
+    return out, stats
+
+
+def attention_bwd(dout, q, k, v, out, stats, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, rel_table=None, bucket_map=None):
+    """Gradients of attention_fwd, which saved out and stats; the probabilities are made again (re_attention_bwd).  -> (dq, dk, dv, dtable): the
+    inputs' shapes and type, laid out as [B, S, H, D]; dtable in rel_table's type (None without one).  Run to run the same bits."""
+    d = _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_table, bucket_map)
+    B, Hq, Sq, D = q.shape
+    Hkv, Sk = k.shape[1], k.shape[2]
+    o_st, g_st = _rows4(out, "out", q)[1], _rows4(dout, "dout", q)[1]
+    _req_any(stats, "stats", q.device, torch.float32)
+    if out.shape != q.shape or dout.shape != q.shape or stats.shape != (2, B, Hq, Sq):
+        raise ValueError("recengine: `out` and `dout` must have q's shape, `stats` [2, batch, heads, rows]")
+    dtable = None if rel_table is None else torch.empty_like(rel_table)
+    dq, dk, dv = _heads_of(B, Sq, Hq, D, q), _heads_of(B, Sk, Hkv, D, q), _heads_of(B, Sk, Hkv, D, q)
+    if not q.numel():                     # no row: nothing reaches the keys
+        for t in (dk, dv) + (() if dtable is None else (dtable,)):
+            t.zero_()
+        return dq, dk, dv, dtable
+    L = lib.load()
+    p = ctypes.addressof(d)
+    ws = _ws(L.re_attention_bwd_workspace_bytes(p), q.device)
+    _call(q.device, L.re_attention_bwd, "re_attention_bwd", p, _a(out), o_st, _a(stats), _a(dout), g_st, _a(dq), _STRIDE3(*dq.stride()[:3]), _a(dk),
+          _STRIDE3(*dk.stride()[:3]), _a(dv), _STRIDE3(*dv.stride()[:3]), _a(dtable), _a(ws), ws.numel())
+    return dq, dk, dv, dtable
