@@ -7,12 +7,15 @@ written against torch / FreeRec picks up the HIP kernels withou
     einsum("BD,ND->BN") full scores     (SASRec/main.py:228, MF-BPR/main.py:104)      score_full
     Adj @ X                             (LightGCN/main.py:80-84)                      spmm_sym
     freerec.criterions.{BPRLoss,BCELoss4Logits}  on logits                            BPRLoss / BCELoss4Logits (restated from call sites)
+    nn.LayerNorm / the elementwise norm          (FMLP-Rec/modules.py:27-40)          layer_norm / LayerNorm (also behind a residual sum)
+    softmax(q k^T / sqrt(D) + mask) v            (BSARec/modules.py:83-143)           attention; with a learned relative_bias / RelativePositionBias
 
 Forward and backward both run through the C ABI (recboard_amd.ops); there is no CPU fallback -- CPU tensors raise.  The engines
 in sasrec.py / gen.py / deepfm.py remain the fast path (fused steps, one arena, hipGraph replay); these ops are the drop-in path.
 """
 import torch
 
+from . import ops
 from . import torch_ops  # noqa: F401  (registers torch.ops.recengine.*)
 from .capture import recording
 
@@ -114,6 +117,63 @@ class Linear(torch.nn.Module):
 
     def forward(self, x):
         return linear(x, self.weight, self.bias)
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
+    """Layer norm over the last dimension: one pass each way, fp32 / bf16 / fp16.  With `residual`: the norm of x + residual -> (y, sum), the sum
+    being the residual stream that goes on (its gradient joins the norm's)."""
+    if residual is None:
+        return _R.layer_norm(x, weight, bias, float(eps))[0]
+    return _R.add_layer_norm(x, residual, weight, bias, float(eps))[:2]
+
+
+class LayerNorm(torch.nn.Module):
+    """Drop-in for torch.nn.LayerNorm(size, eps, elementwise_affine, bias) over the last dimension; forward(x, residual) -> (y, x + residual)."""
+
+    def __init__(self, size, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
+        super().__init__()
+        self.size, self.eps = int(size), eps
+        self.weight = torch.nn.Parameter(torch.ones(self.size, device=device, dtype=dtype)) if elementwise_affine else None
+        self.bias = torch.nn.Parameter(torch.zeros(self.size, device=device, dtype=dtype)) if elementwise_affine and bias else None
+
+    def forward(self, x, residual=None):
+        return layer_norm(x, self.weight, self.bias, self.eps, residual)
+
+
+def relative_bias(table, bucket_map, queries, keys, offset=None):
+    """[H, queries, keys] position bias from the table [buckets, H] (`ops.relative_buckets` makes the map); differentiable in the table."""
+    return _R.relative_bias(table, bucket_map, int(queries), int(keys), int(keys) - int(queries) if offset is None else int(offset))
+
+
+class RelativePositionBias(torch.nn.Module):
+    """A learned bias for each head and bucket of the distance key - query.  forward(queries, keys) is the bias itself; handed to `attention`
+    as `position`, it is made inside, and so is its gradient: no [H, queries, keys] tensor either way."""
+
+    def __init__(self, num_heads, num_buckets=32, max_distance=128, bidirectional=True, device="cuda", dtype=None):
+        super().__init__()
+        self.weight = torch.nn.Parameter(torch.zeros(num_buckets, num_heads, device=device, dtype=dtype))
+        self.register_buffer("bucket_map", ops.relative_buckets(num_buckets, max_distance, bidirectional, device=device), persistent=False)
+
+    def forward(self, queries, keys, offset=None):
+        return relative_bias(self.weight, self.bucket_map, queries, keys, offset)
+
+
+def attention(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, position=None):
+    """softmax(scale q k^T + bias + mask) v, differentiable in q, k, v and the position table: q [B, H, Sq, D], k and v [B, Hkv, Sk, D] (Hkv a divisor of
+    H), D <= 128, arguments as in `ops.attention_fwd`; position: a RelativePositionBias.  A row that sees no key gives 0.
+    The probabilities are not dropped out: a model that does that keeps its own product."""
+    if mask is not None and mask.requires_grad:
+        raise ValueError("recengine: `mask` takes no gradient (a learned bias by distance: `position`)")
+    at = torch.is_tensor(q_offset)
+    return _R.attention(q, k, v, 0.0 if scale is None else _positive(scale), bool(causal), mask, key_lengths, q_offset if at else None,
+                        0 if at else k.shape[2] - q.shape[2] if q_offset is None else int(q_offset), None if position is None else position.weight,
+                        None if position is None else position.bucket_map)[0]
+
+
+def _positive(scale):
+    if not float(scale) > 0.0:
+        raise ValueError("recengine: `scale` must be positive")
+    return float(scale)
 
 
 class _SpmmGeneral(torch.autograd.Function):

@@ -1584,8 +1584,8 @@ def layer_norm_fwd(x, weight=None, bias=None, eps=1e-5, residual=None):
             raise ValueError("recengine: `residual` must have x's shape")
         s = torch.empty_like(x)
     rows = x.numel() // D
-    stats = torch.empty((2,) + x.shape[:-1], dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
     _call(x.device, lib.load().re_layer_norm_fwd, "re_layer_norm_fwd", _a(x), _a(residual), _a(weight), _a(bias), rows, D, float(eps), code, wtype,
           _a(y), _a(s) if residual is not None else None, _a(mean), _a(rstd))
     return y, s, mean, rstd
@@ -1612,8 +1612,8 @@ def layer_norm_bwd(dy, s, weight, mean, rstd, dsum=None, weight_grads=True):
     L = lib.load()
     dw = db = ws = None
     if weight_grads:
-        grads = torch.empty((2, D), dtype=torch.float32 if weight is None else weight.dtype, device=s.device)
-        dw, db = grads[0], grads[1]
+        dw = torch.empty((D,), dtype=torch.float32 if weight is None else weight.dtype, device=s.device)
+        db = torch.empty_like(dw)
         ws = _ws(L.re_layer_norm_bwd_workspace_bytes(rows, D), s.device)
     _call(s.device, L.re_layer_norm_bwd, "re_layer_norm_bwd", _a(dy), _a(s), _a(weight), _a(mean), _a(rstd), _a(dsum), rows, D, code, wtype, _a(ds),
           _a(dw), _a(db), _a(ws), 0 if ws is None else ws.numel())
@@ -1765,7 +1765,7 @@ def _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_tab
 
 def _heads_of(B, S, H, D, like):
     """An empty [B, H, S, D] whose memory is [B, S, H, D]: what the output projection (and a joint q / k / v projection) reads as rows."""
-    return torch.empty((B, S, H, D), dtype=like.dtype, device=like.device).transpose(1, 2)
+    return torch.empty_strided((B, H, S, D), (S * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
 
 
 def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, rel_table=None, bucket_map=None):

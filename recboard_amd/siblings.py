@@ -27,10 +27,12 @@ DeepFM additionally have hand-fused engines (sasrec.py, gen.py, deepfm.py).
   NARM    (NARM/main.py:30-180)    item lookup = recengine::gather_rows, a_1 / a_2 / v_t / b = recengine::gemm, the state at the last real position
                                    = recengine::gather_rows, BCE on gathered rows; the GRU is torch.nn.GRU (MIOpen)
   FMLP-Rec (FMLP-Rec/main.py:38-180, modules.py:27-120) item lookup = recengine::gather_rows, dense_1 / dense_2 of every block = recengine::gemm,
-                                   criteria / ranking as GRU4Rec; the frequency-domain filter is torch.fft (rocFFT)
+                                   criteria / ranking as GRU4Rec; the norms = recengine::layer_norm / add_layer_norm; the frequency-domain filter is
+                                   torch.fft (rocFFT)
   BSARec  (BSARec/main.py:38-200, modules.py:28-200) item lookup = recengine::gather_rows; query / key / value / dense of the attention branch and
                                    dense_1 / dense_2 of the feed-forward = recengine::gemm; criteria / ranking as GRU4Rec; the low-pass branch is
-                                   torch.fft (rocFFT), the S x S attention of a 50-item sequence stays with aten
+                                   torch.fft (rocFFT); the attention is recengine::attention (evaluation, and training without dropped
+                                   probabilities), every norm behind a residual recengine::add_layer_norm
   BERT4Rec (BERT4Rec/main.py:33-195) item lookup = recengine::gather_rows (padding row without gradient), the encoder states at the MASKED
                                    positions = recengine::gather_rows, the projection to the N + 2 logits (`fc`) = recengine::gemm on those
                                    rows only (the reference projects all B*S rows and then selects), full ranking = recengine::gemm on the
@@ -478,7 +480,7 @@ class BERT4Rec(torch.nn.Module):
         self.N, self.maxlen, self.mask_ratio = num_items, maxlen, mask_ratio
         self.item = rnn.Embedding(num_items + self.NUM_PADS, embedding_dim, padding_idx=self.PADDING_VALUE, device=device)
         self.Position = torch.nn.Embedding(maxlen, embedding_dim, device=device)
-        self.layernorm = torch.nn.LayerNorm(embedding_dim, device=device)
+        self.layernorm = rnn.LayerNorm(embedding_dim, device=device)
         self.dropout = torch.nn.Dropout(dropout_rate)
         self.encoder = torch.nn.TransformerEncoder(
             torch.nn.TransformerEncoderLayer(d_model=embedding_dim, nhead=num_heads, dim_feedforward=embedding_dim * 4, dropout=dropout_rate,
@@ -693,10 +695,10 @@ class _TFLayerNorm(torch.nn.Module):
         self.bias = torch.nn.Parameter(torch.zeros(size, device=device))
         self.eps = eps
 
-    def forward(self, x):
-        u = x.mean(-1, keepdim=True)
-        s = (x - u).pow(2).mean(-1, keepdim=True)
-        return self.weight * ((x - u) / torch.sqrt(s + self.eps)) + self.bias
+    def forward(self, x, residual=None):
+        """The norm of x, or of x + residual."""
+        y = rnn.layer_norm(x, self.weight, self.bias, self.eps, residual)
+        return y if residual is None else y[0]
 
 
 class _FilterBlock(torch.nn.Module):
@@ -715,10 +717,10 @@ class _FilterBlock(torch.nn.Module):
     def forward(self, x):
         S = x.shape[1]
         f = torch.fft.irfft(torch.fft.rfft(x, dim=1, norm="ortho") * torch.view_as_complex(self.complex_weight), n=S, dim=1, norm="ortho")
-        h = self.filter_norm(self.dropout(f) + x)
+        h = self.filter_norm(self.dropout(f), x)
         z = _lin3(self.dense_1, h)
         z = z * 0.5 * (1.0 + torch.erf(z / 2.0 ** 0.5))
-        return self.out_norm(self.dropout(_lin3(self.dense_2, z)) + h)
+        return self.out_norm(self.dropout(_lin3(self.dense_2, z)), h)
 
 
 class FMLPRec(_EncodeRanking, torch.nn.Module):
@@ -775,7 +777,7 @@ class _BSAFrequency(torch.nn.Module):
         f = torch.fft.rfft(x, dim=1, norm="ortho")
         f = torch.cat((f[:, :self.c], torch.zeros_like(f[:, self.c:])), dim=1)
         low = torch.fft.irfft(f, n=S, dim=1, norm="ortho")
-        return self.LayerNorm(self.out_dropout(low + self.sqrt_beta ** 2 * (x - low)) + x)
+        return self.LayerNorm(self.out_dropout(low + self.sqrt_beta ** 2 * (x - low)), x)
 
 
 class _BSAAttention(torch.nn.Module):
@@ -785,15 +787,19 @@ class _BSAAttention(torch.nn.Module):
         super().__init__()
         self.H, self.dh = num_heads, D // num_heads
         self.query, self.key, self.value, self.dense = (rnn.Linear(D, D, device=device) for _ in range(4))
-        self.LayerNorm = torch.nn.LayerNorm(D, eps=1e-12, device=device)
+        self.LayerNorm = rnn.LayerNorm(D, eps=1e-12, device=device)
         self.attn_dropout, self.out_dropout = torch.nn.Dropout(attn_dropout_rate), torch.nn.Dropout(hidden_dropout_rate)
 
     def forward(self, x, mask):
         B, S, D = x.shape
         q, k, v = (_lin3(m, x).view(B, S, self.H, self.dh).permute(0, 2, 1, 3) for m in (self.query, self.key, self.value))
-        p = self.attn_dropout(torch.softmax(q @ k.transpose(-1, -2) / self.dh ** 0.5 + mask, dim=-1))
-        ctx = (p @ v).permute(0, 2, 1, 3).reshape(B, S, D)
-        return self.LayerNorm(self.out_dropout(_lin3(self.dense, ctx)) + x)
+        if self.dh > 128 or (self.training and self.attn_dropout.p > 0.0):        # (the engine's attention drops no probabilities)
+            p = self.attn_dropout(torch.softmax(q @ k.transpose(-1, -2) / self.dh ** 0.5 + mask, dim=-1))
+            ctx = p @ v
+        else:
+            ctx = rnn.attention(q, k, v, mask=mask)
+        ctx = ctx.permute(0, 2, 1, 3).reshape(B, S, D)
+        return self.LayerNorm(self.out_dropout(_lin3(self.dense, ctx)), x)[0]
 
 
 class _BSALayer(torch.nn.Module):
@@ -817,7 +823,7 @@ class _BSAFeedForward(torch.nn.Module):
     def forward(self, x):
         z = _lin3(self.dense_1, x)
         z = z * 0.5 * (1.0 + torch.erf(z / 2.0 ** 0.5))
-        return self.LayerNorm(self.dropout(_lin3(self.dense_2, z)) + x)
+        return self.LayerNorm(self.dropout(_lin3(self.dense_2, z)), x)
 
 
 class _BSABlock(torch.nn.Module):
@@ -842,7 +848,7 @@ class BSARec(_EncodeRanking, torch.nn.Module):
         self.N, self.loss_kind = num_items, loss
         self.item = rnn.Embedding(num_items + 1, D, padding_idx=0, device=device)
         self.Position = torch.nn.Embedding(maxlen, D, device=device)
-        self.layerNorm = torch.nn.LayerNorm(D, eps=1e-12, device=device)
+        self.layerNorm = rnn.LayerNorm(D, eps=1e-12, device=device)
         self.embdDropout = torch.nn.Dropout(hidden_dropout_rate)
         self.blocks = torch.nn.ModuleList([_BSABlock(D, num_heads, c, alpha, attn_dropout_rate, hidden_dropout_rate, device) for _ in range(num_blocks)])
         with torch.no_grad():                                    # BSARec.reset_parameters (BSARec/main.py:88-100)

@@ -14,12 +14,18 @@
                                                                            A dY, i.e. it is right for SYMMETRIC A only (the reference's
                                                                            to_normalized_adj("sym")); for any other matrix use
                                                                            recboard_amd.nn.spmm(A, At, X), which takes the transpose explicitly
+    recengine::layer_norm(x, weight, bias, eps) -> (y, mean, rstd)         nn.LayerNorm / the elementwise norm of FMLP-Rec/modules.py:27-40
+    recengine::add_layer_norm(x, residual, weight, bias, eps) -> (y, sum, mean, rstd)      the norm behind a residual sum, in one pass
+    recengine::relative_bias(table, bucket_map, queries, keys, offset) -> Tensor           learned relative position bias by buckets
+    recengine::attention(q, k, v, ...) -> (out, stats)                     softmax attention, nothing of size queries x keys in memory either way
+                                                                           (BSARec/modules.py:83-143)
 
 Each op has a HIP implementation (ctypes -> librecengine.so on the current stream; there is no CPU kernel and CPU tensors raise),
 a fake (meta) implementation so that it traces / exports, and -- where the reference differentiates through it -- a registered
 autograd formula whose backward runs on the engine's kernels too.  `recboard_amd.nn` is the module-level surface over these ops.
 """
 import weakref
+from typing import Optional
 
 import torch
 
@@ -383,6 +389,179 @@ def _bag_bwd(ctx, dE, dfm):
 fm_bag.register_autograd(_bag_bwd, setup_context=_bag_setup)
 
 
+# ---- the operators of a transformer block (fp32 / bf16 / fp16): norm, position bias, attention.  A gradient of an output that nothing used
+#      arrives as None (not as a tensor of zeros), so that the residual form does not read one.
+def _c(t):
+    return None if t is None else t.contiguous()
+
+
+@_lib.custom_op("recengine::layer_norm", mutates_args=(), device_types="cuda")
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+               eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    y, _, mean, rstd = ops.layer_norm_fwd(x.contiguous(), _c(weight), _c(bias), eps)
+    return y, mean, rstd
+
+
+@layer_norm.register_fake
+def _(x, weight, bias, eps=1e-5):
+    stat = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    return torch.empty_like(x, memory_format=torch.contiguous_format), stat, torch.empty_like(stat)
+
+
+@_lib.custom_op("recengine::add_layer_norm", mutates_args=(), device_types="cuda")
+def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[torch.Tensor], bias: Optional[torch.Tensor],
+                   eps: float = 1e-5) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.layer_norm_fwd(x.contiguous(), _c(weight), _c(bias), eps, residual=residual.contiguous())
+
+
+@add_layer_norm.register_fake
+def _(x, residual, weight, bias, eps=1e-5):
+    stat = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    return y, torch.empty_like(y), stat, torch.empty_like(stat)
+
+
+@_lib.custom_op("recengine::layer_norm_backward", mutates_args=(), device_types="cuda")
+def layer_norm_backward(dy: torch.Tensor, s: torch.Tensor, weight: Optional[torch.Tensor], mean: torch.Tensor, rstd: torch.Tensor,
+                        dsum: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    return ops.layer_norm_bwd(dy.contiguous(), s.contiguous(), _c(weight), mean, rstd, dsum=_c(dsum))
+
+
+@layer_norm_backward.register_fake
+def _(dy, s, weight, mean, rstd, dsum):
+    dw = s.new_empty((s.shape[-1],), dtype=torch.float32 if weight is None else weight.dtype)
+    return torch.empty_like(s, memory_format=torch.contiguous_format), dw, torch.empty_like(dw)
+
+
+def _ln_setup(ctx, inputs, output):
+    x, weight, bias, eps = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(x, weight, output[1], output[2])
+    ctx.bias_type = None if bias is None else bias.dtype
+
+
+def _ln_bwd(ctx, dy, dmean, drstd):
+    x, weight, mean, rstd = ctx.saved_tensors
+    if dy is None:
+        return None, None, None, None
+    dx, dw, db = torch.ops.recengine.layer_norm_backward(dy, x, weight, mean, rstd, None)
+    need = ctx.needs_input_grad
+    return dx, dw if need[1] else None, db.to(ctx.bias_type) if need[2] else None, None
+
+
+layer_norm.register_autograd(_ln_bwd, setup_context=_ln_setup)
+
+
+def _aln_setup(ctx, inputs, output):
+    x, residual, weight, bias, eps = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(weight, output[1], output[2], output[3])
+    ctx.bias_type = None if bias is None else bias.dtype
+
+
+def _aln_bwd(ctx, dy, dsum, dmean, drstd):
+    weight, s, mean, rstd = ctx.saved_tensors
+    if dy is None:                                       # only the sum was used
+        return dsum, dsum, None, None, None
+    ds, dw, db = torch.ops.recengine.layer_norm_backward(dy, s, weight, mean, rstd, dsum)
+    need = ctx.needs_input_grad
+    return ds, ds, dw if need[2] else None, db.to(ctx.bias_type) if need[3] else None, None
+
+
+add_layer_norm.register_autograd(_aln_bwd, setup_context=_aln_setup)
+
+
+@_lib.custom_op("recengine::relative_bias", mutates_args=(), device_types="cuda")
+def relative_bias(table: torch.Tensor, bucket_map: torch.Tensor, queries: int, keys: int, offset: int) -> torch.Tensor:
+    return ops.relative_bias_fwd(table.contiguous(), bucket_map, queries, keys, offset)
+
+
+@relative_bias.register_fake
+def _(table, bucket_map, queries, keys, offset):
+    return table.new_empty((table.shape[1], queries, keys))
+
+
+@_lib.custom_op("recengine::relative_bias_backward", mutates_args=(), device_types="cuda")
+def relative_bias_backward(dbias: torch.Tensor, bucket_map: torch.Tensor, buckets: int, offset: int) -> torch.Tensor:
+    return ops.relative_bias_bwd(dbias.contiguous(), bucket_map, buckets, offset)
+
+
+@relative_bias_backward.register_fake
+def _(dbias, bucket_map, buckets, offset):
+    return dbias.new_empty((buckets, dbias.shape[0]))
+
+
+def _rb_setup(ctx, inputs, output):
+    table, bucket_map, queries, keys, offset = inputs
+    ctx.save_for_backward(bucket_map)
+    ctx.buckets, ctx.offset = table.shape[0], offset
+
+
+def _rb_bwd(ctx, dbias):
+    return torch.ops.recengine.relative_bias_backward(dbias, ctx.saved_tensors[0], ctx.buckets, ctx.offset), None, None, None, None
+
+
+relative_bias.register_autograd(_rb_bwd, setup_context=_rb_setup)
+
+
+def _rows(t):
+    """A row's elements adjacent (a view that is not that gets a copy)."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+# scale 0: 1 / sqrt(D); q_offsets (a tensor) goes before q_offset
+@_lib.custom_op("recengine::attention", mutates_args=(), device_types="cuda")
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool, mask: Optional[torch.Tensor],
+              key_lengths: Optional[torch.Tensor], q_offsets: Optional[torch.Tensor], q_offset: int, table: Optional[torch.Tensor],
+              bucket_map: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.attention_fwd(_rows(q), _rows(k), _rows(v), scale=scale or None, causal=causal, mask=mask, key_lengths=key_lengths,
+                             q_offset=q_offset if q_offsets is None else q_offsets, rel_table=_c(table), bucket_map=bucket_map)
+
+
+def _heads_like(t):
+    B, H, S, D = t.shape
+    return t.new_empty_strided((B, H, S, D), (S * H * D, D, H * D, 1))
+
+
+@attention.register_fake
+def _(q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map):
+    return _heads_like(q), q.new_empty((2,) + tuple(q.shape[:3]), dtype=torch.float32)
+
+
+@_lib.custom_op("recengine::attention_backward", mutates_args=(), device_types="cuda")
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor, stats: torch.Tensor, scale: float,
+                       causal: bool, mask: Optional[torch.Tensor], key_lengths: Optional[torch.Tensor], q_offsets: Optional[torch.Tensor],
+                       q_offset: int, table: Optional[torch.Tensor], bucket_map: Optional[torch.Tensor]) -> list[torch.Tensor]:
+    g = ops.attention_bwd(_rows(dout), _rows(q), _rows(k), _rows(v), out, stats, scale=scale or None, causal=causal, mask=mask, key_lengths=key_lengths,
+                          q_offset=q_offset if q_offsets is None else q_offsets, rel_table=_c(table), bucket_map=bucket_map)
+    return [t for t in g if t is not None]
+
+
+@attention_backward.register_fake
+def _(dout, q, k, v, out, stats, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map):
+    g = [_heads_like(q), _heads_like(k), _heads_like(v)]
+    return g if table is None else g + [torch.empty_like(table, memory_format=torch.contiguous_format)]
+
+
+def _attn_setup(ctx, inputs, output):
+    q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map = inputs
+    ctx.set_materialize_grads(False)
+    ctx.save_for_backward(q, k, v, output[0], output[1], mask, key_lengths, q_offsets, table, bucket_map)
+    ctx.scale, ctx.causal, ctx.q_offset = scale, causal, q_offset
+
+
+def _attn_bwd(ctx, dout, dstats):
+    if dout is None:
+        return (None,) * 11
+    q, k, v, out, stats, mask, key_lengths, q_offsets, table, bucket_map = ctx.saved_tensors
+    g = torch.ops.recengine.attention_backward(dout, q, k, v, out, stats, ctx.scale, ctx.causal, mask, key_lengths, q_offsets, ctx.q_offset, table,
+                                               bucket_map)
+    return g[0], g[1], g[2], None, None, None, None, None, None, g[3] if table is not None else None, None
+
+
+attention.register_autograd(_attn_bwd, setup_context=_attn_setup)
+
+
 def _no_cpu(name):
     def raiser(*a, **k):
         raise RuntimeError(f"recengine::{name}: tensors must be on a HIP device (no CPU fallback exists)")
@@ -392,5 +571,8 @@ def _no_cpu(name):
 for _name, _op in (("gather_rows", gather_rows), ("scatter_add_rows", scatter_add_rows), ("bpr_triplet", bpr_triplet),
                    ("bpr_triplet_backward", bpr_triplet_backward), ("score_dense", score_dense), ("gemm", gemm), ("score_topk", score_topk),
                    ("spmm_csr", spmm_csr), ("sasrec_encoder", sasrec_encoder), ("sasrec_encoder_backward", sasrec_encoder_backward),
-                   ("bce_pair", bce_pair), ("bce_pair_backward", bce_pair_backward), ("fm_bag", fm_bag), ("fm_bag_backward", fm_bag_backward)):
+                   ("bce_pair", bce_pair), ("bce_pair_backward", bce_pair_backward), ("fm_bag", fm_bag), ("fm_bag_backward", fm_bag_backward),
+                   ("layer_norm", layer_norm), ("add_layer_norm", add_layer_norm), ("layer_norm_backward", layer_norm_backward),
+                   ("relative_bias", relative_bias), ("relative_bias_backward", relative_bias_backward), ("attention", attention),
+                   ("attention_backward", attention_backward)):
     _op.register_kernel("cpu")(_no_cpu(_name))      # a CPU call fails loudly, with the engine's own message
