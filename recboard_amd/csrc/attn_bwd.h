@@ -10,6 +10,8 @@ struct bwd_io {
     int64_t os[3], dos[3], dqs[3], dks[3], dvs[3];
     const float* stats;            // the forward's [max, log sum][B][Hq][Sq]
     float* delta;                  // [B][Hq][Sq]: rowsum(dO O), written by the dq kernel, read by the dk / dv kernel
+    float* kv_part;                // [splits][dk, dv][B][Hkv][Sk][D], fp32; null: one split
+    int32_t splits;                // parts of the queries (of all heads that share a key head)
     float* part;                   // [B][Hq][tiles][buckets]: the bias gradient of a workgroup; null: none wanted
 };
 struct bwd_plan {
@@ -17,6 +19,7 @@ struct bwd_plan {
     int dp;
     bool mod, vec;
     int64_t qtiles, ktiles;
+    int splits;
     size_t lds_q, lds_k;
 };
 

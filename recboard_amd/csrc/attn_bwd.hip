@@ -6,13 +6,20 @@ namespace attn {
 static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_table) {
     bwd_plan p{};
     p.vec = vec;
-    p.mod = a.table || a.mkind >= 2;
+    p.mod = attn_mod(a);
     p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
     p.wq = a.Sq <= 64 ? 2 : 4;
     p.wk = a.Sk <= 64 ? 2 : 4;
     p.qtiles = re_cdiv(a.Sq, 32 * p.wq);
     p.ktiles = re_cdiv(a.Sk, 32 * p.wk);
     const int rows = dtype == RE_F32 ? 32 : 64;
+    // dk, dv: enough workgroups to fill the card twice over (with a triangle, whose workgroups are uneven, four times), each with eight tiles of
+    // queries at least
+    const int64_t wgs = (int64_t)a.B * a.Hkv * p.ktiles, want = a.causal ? 1024 : 512;
+    int64_t splits = p.ktiles == 0 || wgs >= want ? 1 : re_cdiv(want, wgs);
+    const int64_t most = (int64_t)a.group * re_cdiv(a.Sq, rows) / 8;
+    splits = splits < most ? splits : most;
+    p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
     const int ch = p.dp * (int)re_dtype_size(dtype) / 16;
     const int chp = dtype == RE_F32 ? ch + 1 : ch <= 4 ? 4 : ch <= 8 ? 8 : 16;
     const size_t tiles = (size_t)4 * rows * chp * 16, n_line = 2 * a.R + 1;
@@ -21,6 +28,9 @@ static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_tabl
     return p;
 }
 static size_t delta_bytes(const args& a) { return re_align((size_t)a.B * a.Hq * a.Sq * sizeof(float)); }
+static size_t kv_bytes(const args& a, const bwd_plan& p) {
+    return p.splits > 1 ? re_align((size_t)p.splits * 2 * a.B * a.Hkv * a.Sk * a.D * sizeof(float)) : 0;
+}
 static size_t part_bytes(const args& a, const bwd_plan& p) { return (size_t)a.B * a.Hq * p.qtiles * a.buckets * sizeof(float); }
 
 }  // namespace attn
@@ -28,7 +38,8 @@ static size_t part_bytes(const args& a, const bwd_plan& p) { return (size_t)a.B 
 extern "C" size_t re_attention_bwd_workspace_bytes(const re_attention* d) {
     attn::args a;
     if (attn_args(d, a) != RE_OK || attn_empty(a)) return 0;
-    return attn::delta_bytes(a) + (a.table ? attn::part_bytes(a, attn::make_bwd_plan(a, d->dtype, false, true)) : 0);
+    const attn::bwd_plan p = attn::make_bwd_plan(a, d->dtype, false, true);
+    return attn::delta_bytes(a) + attn::kv_bytes(a, p) + (a.table ? attn::part_bytes(a, p) : 0);
 }
 
 extern "C" int re_attention_bwd(const re_attention* d, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
@@ -43,10 +54,11 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
     const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}, {dout, dout_stride}, {dq, dq_stride},
                                                 {dk, dk_stride}, {dv, dv_stride}});
     const attn::bwd_plan p = attn::make_bwd_plan(a, d->dtype, vec, dtable != nullptr);
-    if ((int64_t)a.B * a.Hq * p.qtiles >= (1ll << 23) || (int64_t)a.B * a.Hkv * p.ktiles >= (1ll << 23)) return RE_EUNSUPPORTED;
-    const size_t need = attn::delta_bytes(a) + (dtable ? attn::part_bytes(a, p) : 0);
+    if ((int64_t)a.B * a.Hq * p.qtiles >= (1ll << 23) || (int64_t)a.B * a.Hkv * p.ktiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
+    const size_t kv = attn::kv_bytes(a, p), need = attn::delta_bytes(a) + kv + (dtable ? attn::part_bytes(a, p) : 0);
     if (!ws || ws_bytes < need) return RE_EWORKSPACE;
-    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, dtable ? (float*)((char*)ws + attn::delta_bytes(a)) : nullptr};
+    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, kv ? (float*)((char*)ws + attn::delta_bytes(a)) : nullptr, p.splits,
+                     dtable ? (float*)((char*)ws + attn::delta_bytes(a) + kv) : nullptr};
     for (int x = 0; x < 3; ++x) {
         io.os[x] = out_stride[x];
         io.dos[x] = dout_stride[x];

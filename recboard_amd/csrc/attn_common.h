@@ -88,36 +88,53 @@ struct tile {
     static constexpr size_t bytes(int rows) { return (size_t)rows * CHP * 16; }
 };
 
-// ROWS x DP elements of a tensor, through the registers of THREADS lanes: load() issues, store() writes to LDS.  Rows from `rows` on and
-// columns from D on are zero and not read.  VEC: every row starts on 16 bytes and D is whole chunks; otherwise element by element.
+// ROWS x DP elements of a tensor into a tile, in two steps: fetch() starts the loads, land() ends them in LDS; a barrier that waits for
+// memory (re_sync_full) comes behind land().
+// 16-bit types on whole 16-byte chunks (VEC) go straight from memory to LDS, the tile's exclusive or applied to the source; no
+// register holds them.  Rows from `rows` on are copies of the last one and columns from D on of the row's last chunk: finite wherever the rows
+// themselves are, and every use of them is multiplied by zero or thrown away.
+// Otherwise through registers, missing rows and columns zero; VEC: chunk by chunk, else element by element.
 template <class T, int DP, int ROWS, int THREADS, bool VEC>
 struct stage {
     typedef tile<T, DP> tl;
-    static constexpr int N = ROWS * tl::CH / THREADS;
-    static_assert(ROWS * tl::CH % THREADS == 0, "whole chunks for each lane");
-    uint4 r[N];
-    __device__ __forceinline__ void load(const T* base, int64_t stride, int rows, int D) {
+    static constexpr bool DIRECT = VEC && sizeof(T) == 2;
+    static constexpr int CH = DIRECT ? tl::CHP : tl::CH;
+    static constexpr int N = ROWS * CH / THREADS;
+    static_assert(ROWS * CH % THREADS == 0, "whole chunks for each lane");
+    uint4 r[DIRECT ? 1 : N];
+    __device__ __forceinline__ void fetch(const T* base, int64_t stride, int rows, int D, T* lds) {
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            const int c = n * THREADS + (int)threadIdx.x, row = c / tl::CH, e = (c % tl::CH) * tl::EPC;
-            r[n] = make_uint4(0, 0, 0, 0);
-            if constexpr (VEC) {
-                if (row < rows && e < D) r[n] = *reinterpret_cast<const uint4*>(base + row * stride + e);
+            const int c = n * THREADS + (int)threadIdx.x, row = c / CH;
+            if constexpr (DIRECT) {
+                const int e = min(((c % CH) ^ tl::swz(row)) * tl::EPC, D - tl::EPC);
+                const uint32_t at = (uint32_t)min(row, rows - 1) * ((uint32_t)stride * 2u) + (uint32_t)e * 2u;      // bytes (vec: below 2^31)
+                const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+                __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(reinterpret_cast<const char*>(base) + at),
+                                                 (__attribute__((address_space(3))) uint32_t*)(lds + (n * THREADS + wave * 64) * tl::EPC), 16, 0, 0);
             } else {
-                union { uint4 u; T t[tl::EPC]; } x;
-                x.u = r[n];
+                const int e = (c % CH) * tl::EPC;
+                r[n] = make_uint4(0, 0, 0, 0);
+                if constexpr (VEC) {
+                    if (row < rows && e < D) r[n] = *reinterpret_cast<const uint4*>(base + row * stride + e);
+                } else {
+                    union { uint4 u; T t[tl::EPC]; } x;
+                    x.u = r[n];
 #pragma unroll
-                for (int i = 0; i < tl::EPC; ++i)
-                    if (row < rows && e + i < D) x.t[i] = base[row * stride + e + i];
-                r[n] = x.u;
+                    for (int i = 0; i < tl::EPC; ++i)
+                        if (row < rows && e + i < D) x.t[i] = base[row * stride + e + i];
+                    r[n] = x.u;
+                }
             }
         }
     }
-    __device__ __forceinline__ void store(T* lds) const {
+    __device__ __forceinline__ void land(T* lds) const {
+        if constexpr (!DIRECT) {
 #pragma unroll
-        for (int n = 0; n < N; ++n) {
-            const int c = n * THREADS + (int)threadIdx.x;
-            *reinterpret_cast<uint4*>(lds + tl::at(c / tl::CH, c % tl::CH)) = r[n];
+            for (int n = 0; n < N; ++n) {
+                const int c = n * THREADS + (int)threadIdx.x;
+                *reinterpret_cast<uint4*>(lds + tl::at(c / CH, c % CH)) = r[n];
+            }
         }
     }
 };
@@ -248,7 +265,8 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) < ATTN_INF); }
 
-// A 32 x 32 block of raw products -> scores (MOD: bias or additive mask) or the products as they are (otherwise), shut places -inf.  Scores stay
+// A 32 x 32 block of raw products -> scores (MOD: with a bias, or with a mask that is additive or differs between rows) or the products as they
+// are (otherwise: lengths, the triangle, truth values by key), shut places -inf.  Scores stay
 // in natural units: a mask of the type's lowest value would overflow as a multiple of log2 e, and a row that holds nothing else has
 // to come out even.
 // The lane's column is query (i, h) and rows are keys j0 + row_of (BY_KEY = false), or the column is key j and rows are queries (true).
@@ -265,14 +283,17 @@ __device__ __forceinline__ void apply_keys(const args& a, f32x16& s, int b, int 
             for (int r = 0; r < 16; ++r) s[r] += line[clip_distance(d0 + row_of(r, half), a.R) + a.R];
         }
     }
-    if (a.mkind && !mask_by_key(a)) {
-        const int64_t at = b * a.ms[0] + h * a.ms[1] + (int64_t)i * a.ms[2] + (int64_t)j0 * a.ms[3];
+    if constexpr (MOD) {
+        if (a.mkind && !mask_by_key(a)) {
+            int64_t at = b * a.ms[0] + h * a.ms[1] + (int64_t)i * a.ms[2] + (int64_t)j0 * a.ms[3];
+            asm volatile("" : "+v"(at));               // (sixteen addresses carried from tile to tile would not fit the registers)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int row = row_of(r, half);
-            if (bits >> row & 1) {                      // (a key that is there: its mask may be read)
-                const float m = mask_add(a, at + row * a.ms[3]);
-                s[r] = m == -ATTN_INF ? -ATTN_INF : MOD ? s[r] + m : s[r];
+            for (int r = 0; r < 16; ++r) {
+                const int row = row_of(r, half);
+                if (bits >> row & 1) {                  // (a key that is there: its mask may be read)
+                    const float m = mask_add(a, at + row * a.ms[3]);
+                    s[r] = m == -ATTN_INF ? -ATTN_INF : s[r] + m;
+                }
             }
         }
     }
@@ -286,18 +307,19 @@ __device__ __forceinline__ void apply_keys(const args& a, f32x16& s, int b, int 
         for (int r = 0; r < 16; ++r) s[r] = row_of(r, half) > last ? -ATTN_INF : s[r];
     }
 }
+// 2^x as the one instruction: x <= 8 here, and below -126 the result is taken as 0 (the library's form pays four more instructions for denormals)
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // exp(s - m) of a block's score; mu: m in natural units (MOD) or m * scale * log2 e of the products' units
 template <bool MOD>
 __device__ __forceinline__ float exp_of(float s, float mu, float c1) {
-    if constexpr (MOD) return exp2f((s - mu) * ATTN_LOG2E);
-    else return exp2f(s * c1 - mu);
+    if constexpr (MOD) return exp2_fast((s - mu) * ATTN_LOG2E);
+    else return exp2_fast(s * c1 - mu);
 }
-// bits of keys j0 .. j0 + 63 that are there; every lane of a wave calls it
-__device__ __forceinline__ uint64_t key_bits(const args& a, int b, int j0, int len, bool by_key, int lane) {
-    const int j = j0 + lane;
+// May anything see key j (length, by-key mask)?  A wave's answers for 64 keys are the bits of apply_keys.
+__device__ __forceinline__ bool key_there(const args& a, int b, int j, int len, bool by_key) {
     bool there = j < len;
     if (there && by_key) there = static_cast<const uint8_t*>(a.mask)[b * a.ms[0] + j * a.ms[3]] != 0;
-    return __ballot(there);
+    return there;
 }
 
 }  // namespace attn
@@ -324,11 +346,14 @@ static inline int attn_args(const re_attention* d, attn::args& a) {
 }
 static inline bool attn_empty(const attn::args& a) { return a.B == 0 || a.Hq == 0 || a.Sq == 0; }
 
+// the kernels' general form: scores are formed place by place
+static inline bool attn_mod(const attn::args& a) { return a.table || a.mkind >= 2 || (a.mkind == 1 && (a.ms[1] || a.ms[2])); }
+
 struct attn_tensor {
     const void* p;
     const int64_t* stride;
 };
-// every row of every tensor starts on 16 bytes, and is whole 16-byte chunks
+// every row of every tensor starts on 16 bytes and is whole 16-byte chunks, and rows are not gigabytes apart
 static inline bool attn_aligned(const attn::args& a, int32_t dtype, std::initializer_list<attn_tensor> ts) {
     const int64_t epc = 16 / (int64_t)re_dtype_size(dtype);
     if (a.D % epc) return false;
@@ -336,6 +361,7 @@ static inline bool attn_aligned(const attn::args& a, int32_t dtype, std::initial
         if (reinterpret_cast<uintptr_t>(t.p) & 15) return false;
         for (int x = 0; x < 3; ++x)
             if (t.stride[x] % epc) return false;
+        if (t.stride[2] > (1 << 22)) return false;      // (a tile's rows lie within 2^31 bytes: 32-bit offsets)
     }
     return true;
 }

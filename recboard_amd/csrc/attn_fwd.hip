@@ -14,7 +14,7 @@ static size_t lds_bytes(int dtype, int dp, int bk, const args& a, int pg) {
 static fwd_plan make_plan(const args& a, int dtype, bool vec) {
     fwd_plan p{};
     p.vec = vec;
-    p.mod = a.table || a.mkind >= 2;
+    p.mod = attn_mod(a);
     p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
     // few rows: the heads that share keys are one workgroup's rows and its waves go along the keys
     const int64_t packed = (int64_t)a.group * a.Sq;
