@@ -9,7 +9,8 @@ struct fwd_out {
     int64_t os[3];                 // batch, head, row
     float* stats;                  // [max, log sum][B][Hq][Sq]
     float* part;                   // [splits][B][Hq][Sq][D], then [splits][B][Hq][Sq][2]; null: one split
-    int32_t splits, tiles, heads, pg, xcd;   // heads: workgroup heads per sequence; pg: query heads that share a workgroup's rows
+    order ord;                     // units: workgroup heads of all sequences; tiles: query tiles x splits
+    int32_t splits, tiles, heads, pg;        // heads: workgroup heads per sequence; pg: query heads that share a workgroup's rows
 };
 
 struct fwd_plan {

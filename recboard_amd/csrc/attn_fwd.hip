@@ -56,9 +56,8 @@ extern "C" int re_attention_fwd(const re_attention* d, void* out, const int64_t*
     const attn::fwd_plan p = attn::make_plan(a, d->dtype, vec);
     if ((int64_t)a.B * p.heads * p.tiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
     if (p.part && (!ws || ws_bytes < p.part)) return RE_EWORKSPACE;
-    const int64_t grid = (int64_t)a.B * p.heads * p.tiles * p.splits;
-    const attn::fwd_out f{out, {out_stride[0], out_stride[1], out_stride[2]}, stats, p.part ? (float*)ws : nullptr, p.splits, p.tiles, p.heads, p.pg,
-                          grid % 8 == 0};
+    const attn::fwd_out f{out, {out_stride[0], out_stride[1], out_stride[2]}, stats, p.part ? (float*)ws : nullptr,
+                          attn_order((int64_t)a.B * p.heads, (int64_t)p.tiles * p.splits), p.splits, p.tiles, p.heads, p.pg};
     re_clear_error();
     hipStream_t st = (hipStream_t)stream;
     const int r = d->dtype == RE_F32 ? attn::fwd_launch<float>(a, f, p, st) : d->dtype == RE_BF16 ? attn::fwd_launch<re_bf16>(a, f, p, st)
