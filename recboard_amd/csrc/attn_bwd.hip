@@ -12,19 +12,22 @@ static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_tabl
     p.wk = a.Sk <= 64 ? 2 : 4;
     p.qtiles = re_cdiv(a.Sq, 32 * p.wq);
     p.ktiles = re_cdiv(a.Sk, 32 * p.wk);
-    const int rows = dtype == RE_F32 ? 32 : 64;
-    // dk, dv: enough workgroups to fill the card twice over (with a triangle, whose workgroups are uneven, four times), each with eight tiles of
-    // queries at least
+    const int rows = dtype == RE_F32 ? 32 : 64;                                      // keys of a dq tile
+    const bool v_lds = dtype != RE_F32 && p.dp > 64;
+    const int qrows = dtype == RE_F32 || v_lds ? 32 : 64;                            // queries of a dk, dv tile
+    // dk, dv: enough workgroups to fill the card twice over (with a triangle, whose workgroups are uneven, four times), each with 512 queries
+    // at least
     const int64_t wgs = (int64_t)a.B * a.Hkv * p.ktiles, want = a.causal ? 1024 : 512;
     int64_t splits = p.ktiles == 0 || wgs >= want ? 1 : re_cdiv(want, wgs);
-    const int64_t most = (int64_t)a.group * re_cdiv(a.Sq, rows) / 8;
+    const int64_t most = (int64_t)a.group * re_cdiv(a.Sq, 64) / 8;
     splits = splits < most ? splits : most;
     p.splits = (int)(splits < 1 ? 1 : splits > 16 ? 16 : splits);
     const int ch = p.dp * (int)re_dtype_size(dtype) / 16;
     const int chp = dtype == RE_F32 ? ch + 1 : ch <= 4 ? 4 : ch <= 8 ? 8 : 16;
     const size_t tiles = (size_t)4 * rows * chp * 16, n_line = 2 * a.R + 1;
-    p.lds_q = tiles + (a.table ? n_line * sizeof(float) : 0) + (want_table ? p.wq * (n_line + 32 * 33) * sizeof(float) : 0);
-    p.lds_k = tiles + 6 * rows * sizeof(float) + (a.table ? n_line * sizeof(float) : 0);
+    const size_t line = a.table ? line_len(a.R) * sizeof(float) : 0;
+    p.lds_q = tiles + line + (want_table ? p.wq * 2 * (n_line + 124) * sizeof(float) : 0);
+    p.lds_k = (size_t)(4 * qrows + (v_lds ? 32 * p.wk : 0)) * chp * 16 + 6 * qrows * sizeof(float) + line;
     return p;
 }
 static size_t delta_bytes(const args& a) { return re_align((size_t)a.B * a.Hq * a.Sq * sizeof(float)); }

@@ -92,15 +92,15 @@ struct tile {
 // memory (re_sync_full) comes behind land().
 // 16-bit types on whole 16-byte chunks (VEC) go straight from memory to LDS, the tile's exclusive or applied to the source; no
 // register holds them.  Rows from `rows` on are copies of the last one and columns from D on of the row's last chunk: finite wherever the rows
-// themselves are, and every use of them is multiplied by zero or thrown away.
-// Otherwise through registers, missing rows and columns zero; VEC: chunk by chunk, else element by element.
-template <class T, int DP, int ROWS, int THREADS, bool VEC>
+// themselves are, and every use of them is multiplied by zero or thrown away: the other operand of a contraction over columns is zero from D on.
+// Otherwise (ZEROS: asked for) through registers, missing rows and columns zero; VEC: chunk by chunk, else element by element.
+template <class T, int DP, int ROWS, int THREADS, bool VEC, bool ZEROS = false>
 struct stage {
     typedef tile<T, DP> tl;
-    static constexpr bool DIRECT = VEC && sizeof(T) == 2;
+    static constexpr bool DIRECT = VEC && !ZEROS && sizeof(T) == 2;
     static constexpr int CH = DIRECT ? tl::CHP : tl::CH;
-    static constexpr int N = ROWS * CH / THREADS;
-    static_assert(ROWS * CH % THREADS == 0, "whole chunks for each lane");
+    static constexpr int N = (ROWS * CH + THREADS - 1) / THREADS;
+    static_assert(!DIRECT || ROWS * CH % THREADS == 0, "whole waves of chunks");
     uint4 r[DIRECT ? 1 : N];
     __device__ __forceinline__ void fetch(const T* base, int64_t stride, int rows, int D, T* lds) {
 #pragma unroll
@@ -116,13 +116,13 @@ struct stage {
                 const int e = (c % CH) * tl::EPC;
                 r[n] = make_uint4(0, 0, 0, 0);
                 if constexpr (VEC) {
-                    if (row < rows && e < D) r[n] = *reinterpret_cast<const uint4*>(base + row * stride + e);
+                    if (row < rows && row < ROWS && e < D) r[n] = *reinterpret_cast<const uint4*>(base + row * stride + e);
                 } else {
                     union { uint4 u; T t[tl::EPC]; } x;
                     x.u = r[n];
 #pragma unroll
                     for (int i = 0; i < tl::EPC; ++i)
-                        if (row < rows && e + i < D) x.t[i] = base[row * stride + e + i];
+                        if (row < rows && row < ROWS && e + i < D) x.t[i] = base[row * stride + e + i];
                     r[n] = x.u;
                 }
             }
@@ -133,7 +133,7 @@ struct stage {
 #pragma unroll
             for (int n = 0; n < N; ++n) {
                 const int c = n * THREADS + (int)threadIdx.x;
-                *reinterpret_cast<uint4*>(lds + tl::at(c / CH, c % CH)) = r[n];
+                if (ROWS * CH % THREADS == 0 || c < ROWS * CH) *reinterpret_cast<uint4*>(lds + tl::at(c / CH, c % CH)) = r[n];
             }
         }
     }
@@ -242,12 +242,14 @@ __device__ __forceinline__ float mask_add(const args& a, int64_t at) {
 }
 __device__ __forceinline__ int clip_distance(int d, int R) { return d < -R ? -R : d > R ? R : d; }
 
-// the bias of `heads` heads from h0 on, [heads][2 R + 1] in LDS
+// A head's bias by distance in LDS: distances -R - 31 .. R + 31, the ends repeated.  A lane's 32 distances in a block then need one clamp, of their
+// lowest, and sixteen constant offsets from it.  `line` points to distance -R.
+__host__ __device__ inline int line_len(int R) { return 2 * R + 63; }
 template <int THREADS>
 __device__ __forceinline__ void load_lines(const args& a, int h0, int heads, float* line) {
-    const int n = 2 * a.R + 1;
+    const int n = line_len(a.R);
     for (int x = threadIdx.x; x < heads * n; x += THREADS)
-        line[x] = rb_entry(a.table, a.tdtype, a.map, x % n, a.buckets, a.Hq, h0 + x / n);
+        line[x - 31] = rb_entry(a.table, a.tdtype, a.map, clip_distance(x % n - 31 - a.R, a.R) + a.R, a.buckets, a.Hq, h0 + x / n);
 }
 
 // Does the mask depend on the key alone (within a sequence)?  Then a tile's part of it is one bit a key.
@@ -280,6 +282,15 @@ __device__ __forceinline__ float wave_max(float v) {
 }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) < ATTN_INF); }
 
+// s[r] += the bias at distance d0 + SIGN * row_of(r)
+template <int SIGN>
+__device__ __forceinline__ void add_bias(f32x16& s, const float* line, int d0, int half, int R) {
+    const int lo = SIGN > 0 ? d0 : d0 - 31;
+    const float* at = line + ((lo < -R - 31 ? -R - 31 : lo > R ? R : lo) + R + (SIGN > 0 ? 4 * half : 31 - 4 * half));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] += at[SIGN * row_of(r, 0)];
+}
+
 // A 32 x 32 block of raw products -> scores (MOD: with a bias, or with a mask that is additive or differs between rows) or the products as they
 // are (otherwise: lengths, the triangle, truth values by key), shut places -inf.  Scores stay
 // in natural units: a mask of the type's lowest value would overflow as a multiple of log2 e, and a row that holds nothing else has
@@ -292,11 +303,7 @@ __device__ __forceinline__ void apply_keys(const args& a, f32x16& s, int b, int 
     if constexpr (MOD) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] *= a.scale;
-        if (a.table) {
-            const int d0 = j0 - (off + i);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] += line[clip_distance(d0 + row_of(r, half), a.R) + a.R];
-        }
+        if (a.table) add_bias<1>(s, line, j0 - (off + i), half, a.R);
     }
     if constexpr (MOD) {
         if (a.mkind && !mask_by_key(a)) {

@@ -7,7 +7,7 @@ static size_t lds_bytes(int dtype, int dp, int bk, const args& a, int pg) {
     const int ch = dp * (int)re_dtype_size(dtype) / 16;
     const int chp = dtype == RE_F32 ? ch + 1 : ch <= 4 ? 4 : ch <= 8 ? 8 : 16;
     size_t n = (size_t)4 * bk * chp * 16;
-    if (a.table) n += (size_t)pg * (2 * a.R + 1) * sizeof(float);
+    if (a.table) n += (size_t)pg * line_len(a.R) * sizeof(float);
     return n;
 }
 
@@ -18,7 +18,7 @@ static fwd_plan make_plan(const args& a, int dtype, bool vec) {
     p.dp = a.D <= 32 ? 32 : a.D <= 64 ? 64 : a.D <= 96 ? 96 : 128;
     // few rows: the heads that share keys are one workgroup's rows and its waves go along the keys
     const int64_t packed = (int64_t)a.group * a.Sq;
-    const bool few = packed <= 32 && (!a.table || (int64_t)a.group * (2 * a.R + 1) <= 4096);
+    const bool few = packed <= 32 && (!a.table || (int64_t)a.group * line_len(a.R) <= 4096);
     p.pg = few ? a.group : 1;
     p.wk = !few && a.Sq > 32 ? 1 : dtype == RE_F32 ? 2 : 4;      // (fp32: 64 keys of 128 elements fill LDS)
     p.wq = p.wk > 1 ? 1 : a.Sq <= 64 ? 2 : 4;
