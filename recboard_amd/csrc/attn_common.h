@@ -88,13 +88,21 @@ struct tile {
     static constexpr size_t bytes(int rows) { return (size_t)rows * CHP * 16; }
 };
 
+// 16 bytes a lane from base + at (bytes) to 64 consecutive pieces of LDS, as the bare instruction (nothing is returned in registers; the wait is the
+// caller's re_sync_full).  Behind the builtin the transposed reads wait for all loads in flight: the tile that was just asked for is then
+// waited for in the middle of the one before, which a kernel of two waves a SIMD hides and a stream over a cache does not.
+__device__ __forceinline__ void to_lds(const void* base, uint32_t at, const void* lds) {
+    const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at), "s"(base) : "memory");
+}
+
 // ROWS x DP elements of a tensor into a tile, in two steps: fetch() starts the loads, land() ends them in LDS; a barrier that waits for
 // memory (re_sync_full) comes behind land().
 // 16-bit types on whole 16-byte chunks (VEC) go straight from memory to LDS, the tile's exclusive or applied to the source; no
 // register holds them.  Rows from `rows` on are copies of the last one and columns from D on of the row's last chunk: finite wherever the rows
 // themselves are, and every use of them is multiplied by zero or thrown away: the other operand of a contraction over columns is zero from D on.
-// Otherwise (ZEROS: asked for) through registers, missing rows and columns zero; VEC: chunk by chunk, else element by element.
-template <class T, int DP, int ROWS, int THREADS, bool VEC, bool ZEROS = false>
+// PLAIN: by the bare instruction.  Otherwise (ZEROS: asked for) through registers, missing rows and columns zero; VEC: chunk by chunk, else element by element.
+template <class T, int DP, int ROWS, int THREADS, bool VEC, bool ZEROS = false, bool PLAIN = false>
 struct stage {
     typedef tile<T, DP> tl;
     static constexpr bool DIRECT = VEC && !ZEROS && sizeof(T) == 2;
@@ -110,8 +118,13 @@ struct stage {
                 const int e = min(((c % CH) ^ tl::swz(row)) * tl::EPC, D - tl::EPC);
                 const uint32_t at = (uint32_t)min(row, rows - 1) * ((uint32_t)stride * 2u) + (uint32_t)e * 2u;      // bytes (vec: below 2^31)
                 const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+                T* const to = lds + (n * THREADS + wave * 64) * tl::EPC;
+                if constexpr (PLAIN) {
+                    to_lds(base, at, to);
+                    continue;
+                }
                 __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(reinterpret_cast<const char*>(base) + at),
-                                                 (__attribute__((address_space(3))) uint32_t*)(lds + (n * THREADS + wave * 64) * tl::EPC), 16, 0, 0);
+                                                 (__attribute__((address_space(3))) uint32_t*)(to), 16, 0, 0);
             } else {
                 const int e = (c % CH) * tl::EPC;
                 r[n] = make_uint4(0, 0, 0, 0);
@@ -210,18 +223,20 @@ __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
 
 // Workgroup -> (unit, tile): a unit is what shares keys and values (a sequence's head), its tiles are work of one kind, with a triangle the
-// longest first.  Workgroups are dealt to the eight XCDs in turn: units stay on one XCD (its L2 holds what they share) where eight divides them,
-// and there `set` units run side by side, tile by tile, so that the long tiles of all of them start before the short ones of any
-// (2 x 16 heads x 4096 x 128, causal: 238 us a head at a time).
+// longest first.  Workgroups are dealt to the eight XCDs in turn: where eight divides the groups of `chunk` units that share keys and values, a
+// group stays on one XCD (its L2 holds what they share), neighbouring groups on neighbouring XCDs (a ragged batch has its long sequence on all
+// of them); and there `set` units run side by side, tile by tile, so that the long tiles of all of them start before the short ones of any
+// (2 x 16 heads x 4096 x 128, causal, forward: 238 us a head at a time, 185 so).
 struct order {
-    int32_t xcd, units, tiles, set;      // xcd: 8, or 1; units per XCD; set divides units
+    int32_t xcd, units, tiles, set, chunk;      // xcd: 8, or 1; units per XCD; set divides units
 };
 __device__ __forceinline__ void place(const order& o, int id, int& unit, int& tile) {
     const int x = id % o.xcd;
     id /= o.xcd;
     const int per = o.set * o.tiles, first = id / per * o.set, r = id % per;
     tile = r / o.set;
-    unit = x * o.units + first + r % o.set;
+    const int l = first + r % o.set;
+    unit = (l / o.chunk * o.xcd + x) * o.chunk + l % o.chunk;
 }
 
 // ---------------------------------------------------------------------------------------------------------- lengths, masks, bias
@@ -337,10 +352,11 @@ __device__ __forceinline__ float exp_of(float s, float mu, float c1) {
     if constexpr (MOD) return exp2_fast((s - mu) * ATTN_LOG2E);
     else return exp2_fast(s * c1 - mu);
 }
-// May anything see key j (length, by-key mask)?  A wave's answers for 64 keys are the bits of apply_keys.
-__device__ __forceinline__ bool key_there(const args& a, int b, int j, int len, bool by_key) {
-    bool there = j < len;
-    if (there && by_key) there = static_cast<const uint8_t*>(a.mask)[b * a.ms[0] + j * a.ms[3]] != 0;
+// May anything see key j (length, by-key mask)?  Not 0: yes.  A wave's answers for 64 keys are the bits of apply_keys; asked for a tile ahead, and
+// kept as the byte that was loaded, so that the load is not waited for before it is used.
+__device__ __forceinline__ int key_there(const args& a, int b, int j, int len, bool by_key) {
+    int there = j < len;
+    if (there && by_key) there = static_cast<const uint8_t*>(a.mask)[b * a.ms[0] + j * a.ms[3]];
     return there;
 }
 
@@ -371,9 +387,10 @@ static inline bool attn_empty(const attn::args& a) { return a.B == 0 || a.Hq == 
 // the kernels' general form: scores are formed place by place
 static inline bool attn_mod(const attn::args& a) { return a.table || a.mkind >= 2 || (a.mkind == 1 && (a.ms[1] || a.ms[2])); }
 
-static inline attn::order attn_order(int64_t units, int64_t tiles) {
+static inline attn::order attn_order(int64_t units, int64_t tiles, int chunk) {
     attn::order o;
-    o.xcd = units % 8 == 0 ? 8 : 1;
+    o.chunk = chunk;
+    o.xcd = units / chunk % 8 == 0 ? 8 : 1;
     o.units = (int32_t)(units / o.xcd);
     o.tiles = (int32_t)tiles;
     // a set fills an XCD's 32 units of two workgroups each twice over

@@ -20,7 +20,7 @@ static fwd_plan make_plan(const args& a, int dtype, bool vec) {
     const int64_t packed = (int64_t)a.group * a.Sq;
     const bool few = packed <= 32 && (!a.table || (int64_t)a.group * line_len(a.R) <= 4096);
     p.pg = few ? a.group : 1;
-    p.wk = !few && a.Sq > 32 ? 1 : dtype == RE_F32 ? 2 : 4;      // (fp32: 64 keys of 128 elements fill LDS)
+    p.wk = !few && a.Sq > 32 ? 1 : 2;
     p.wq = p.wk > 1 ? 1 : a.Sq <= 64 ? 2 : 4;
     p.bk = 32 * (dtype == RE_F32 || p.wk > 1 ? 1 : 2) * p.wk;
     p.heads = p.pg > 1 ? a.Hkv : a.Hq;
@@ -57,7 +57,7 @@ extern "C" int re_attention_fwd(const re_attention* d, void* out, const int64_t*
     if ((int64_t)a.B * p.heads * p.tiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
     if (p.part && (!ws || ws_bytes < p.part)) return RE_EWORKSPACE;
     const attn::fwd_out f{out, {out_stride[0], out_stride[1], out_stride[2]}, stats, p.part ? (float*)ws : nullptr,
-                          attn_order((int64_t)a.B * p.heads, (int64_t)p.tiles * p.splits), p.splits, p.tiles, p.heads, p.pg};
+                          attn_order((int64_t)a.B * p.heads, (int64_t)p.tiles * p.splits, p.pg > 1 ? 1 : a.group), p.splits, p.tiles, p.heads, p.pg};
     re_clear_error();
     hipStream_t st = (hipStream_t)stream;
     const int r = d->dtype == RE_F32 ? attn::fwd_launch<float>(a, f, p, st) : d->dtype == RE_BF16 ? attn::fwd_launch<re_bf16>(a, f, p, st)
