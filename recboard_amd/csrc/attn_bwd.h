@@ -12,14 +12,16 @@ struct bwd_io {
     float* delta;                  // [B][Hq][Sq]: rowsum(dO O), written by the dq kernel, read by the dk / dv kernel
     float* kv_part;                // [splits][dk, dv][B][Hkv][Sk][D], fp32; null: one split
     int32_t splits;                // parts of the queries (of all heads that share a key head)
-    float* part;                   // [B][Hq][tiles][buckets]: the bias gradient of a workgroup; null: none wanted
+    float* q_part;                 // [qsplits][B][Hq][Sq][D], fp32; null: one split
+    int32_t qsplits;               // parts of the keys for dq
+    float* part;                   // [B][Hq][tiles x qsplits][buckets]: the bias gradient of a workgroup; null: none wanted
 };
 struct bwd_plan {
     int wq, wk;                    // waves of the dq / of the dk, dv kernel: 32 queries / 32 keys each
     int dp;
     bool mod, vec;
     int64_t qtiles, ktiles;
-    int splits;
+    int splits, qsplits;           // of the queries for dk, dv; of the keys for dq
     size_t lds_q, lds_k;
 };
 

@@ -15,6 +15,11 @@ static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_tabl
     const int rows = dtype == RE_F32 ? 32 : 64;                                      // keys of a dq tile
     const bool v_lds = dtype != RE_F32 && p.dp > 64;
     const int qrows = dtype == RE_F32 || v_lds ? 32 : 64;                            // queries of a dk, dv tile
+    // dq: two workgroups a compute unit, each with four tiles of keys at least
+    const int64_t qwgs = (int64_t)a.B * a.Hq * p.qtiles, qmost = re_cdiv(a.Sk, 256);
+    int64_t qs = qwgs >= 384 ? 1 : re_cdiv(512, qwgs);
+    qs = qs < qmost ? qs : qmost;
+    p.qsplits = (int)(qs < 1 ? 1 : qs > 16 ? 16 : qs);
     // dk, dv: enough workgroups to fill the card twice over (with a triangle, whose workgroups are uneven, four times), each with 512 queries
     // at least
     const int64_t wgs = (int64_t)a.B * a.Hkv * p.ktiles, want = a.causal ? 1024 : 512;
@@ -34,7 +39,10 @@ static size_t delta_bytes(const args& a) { return re_align((size_t)a.B * a.Hq * 
 static size_t kv_bytes(const args& a, const bwd_plan& p) {
     return p.splits > 1 ? re_align((size_t)p.splits * 2 * a.B * a.Hkv * a.Sk * a.D * sizeof(float)) : 0;
 }
-static size_t part_bytes(const args& a, const bwd_plan& p) { return (size_t)a.B * a.Hq * p.qtiles * a.buckets * sizeof(float); }
+static size_t q_bytes(const args& a, const bwd_plan& p) {
+    return p.qsplits > 1 ? re_align((size_t)p.qsplits * a.B * a.Hq * a.Sq * a.D * sizeof(float)) : 0;
+}
+static size_t part_bytes(const args& a, const bwd_plan& p) { return (size_t)a.B * a.Hq * p.qtiles * p.qsplits * a.buckets * sizeof(float); }
 
 }  // namespace attn
 
@@ -42,7 +50,7 @@ extern "C" size_t re_attention_bwd_workspace_bytes(const re_attention* d) {
     attn::args a;
     if (attn_args(d, a) != RE_OK || attn_empty(a)) return 0;
     const attn::bwd_plan p = attn::make_bwd_plan(a, d->dtype, false, true);
-    return attn::delta_bytes(a) + attn::kv_bytes(a, p) + (a.table ? attn::part_bytes(a, p) : 0);
+    return attn::delta_bytes(a) + attn::kv_bytes(a, p) + attn::q_bytes(a, p) + (a.table ? attn::part_bytes(a, p) : 0);
 }
 
 extern "C" int re_attention_bwd(const re_attention* d, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
@@ -57,11 +65,12 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
     const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}, {dout, dout_stride}, {dq, dq_stride},
                                                 {dk, dk_stride}, {dv, dv_stride}});
     const attn::bwd_plan p = attn::make_bwd_plan(a, d->dtype, vec, dtable != nullptr);
-    if ((int64_t)a.B * a.Hq * p.qtiles >= (1ll << 23) || (int64_t)a.B * a.Hkv * p.ktiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
-    const size_t kv = attn::kv_bytes(a, p), need = attn::delta_bytes(a) + kv + (dtable ? attn::part_bytes(a, p) : 0);
+    if ((int64_t)a.B * a.Hq * p.qtiles * p.qsplits >= (1ll << 23) || (int64_t)a.B * a.Hkv * p.ktiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
+    const size_t kv = attn::kv_bytes(a, p), qb = attn::q_bytes(a, p), need = attn::delta_bytes(a) + kv + qb + (dtable ? attn::part_bytes(a, p) : 0);
     if (!ws || ws_bytes < need) return RE_EWORKSPACE;
-    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, kv ? (float*)((char*)ws + attn::delta_bytes(a)) : nullptr, p.splits,
-                     dtable ? (float*)((char*)ws + attn::delta_bytes(a) + kv) : nullptr};
+    char* at = (char*)ws + attn::delta_bytes(a);
+    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, kv ? (float*)at : nullptr, p.splits, qb ? (float*)(at + kv) : nullptr,
+                    p.qsplits, dtable ? (float*)(at + kv + qb) : nullptr};
     for (int x = 0; x < 3; ++x) {
         io.os[x] = out_stride[x];
         io.dos[x] = dout_stride[x];
@@ -75,7 +84,7 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
                                                                                               : attn::bwd_launch<re_f16>(a, io, p, st);
     if (r != RE_OK) return r;
     if (dtable)
-        hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)a.Hq), dim3(256), 0, st, io.part, (int64_t)a.B, (int64_t)a.Hq, p.qtiles, a.buckets, dtable,
+        hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)a.Hq), dim3(256), 0, st, io.part, (int64_t)a.B, (int64_t)a.Hq, p.qtiles * p.qsplits, a.buckets, dtable,
                            a.tdtype);
     return re_launch_status();
 }

@@ -16,10 +16,12 @@ __device__ __forceinline__ float rb_entry(const void* table, int32_t dtype, cons
     return (unsigned)k < (unsigned)buckets ? re_load_as_float(table, k * H + h, dtype) : 0.f;
 }
 
-// out[k] = the sum of line[d] over the distances in bucket k, by a workgroup of THREADS (line in LDS, complete; `tmp`: THREADS floats of LDS).
-// Fixed order: every bucket is cut into the same slices whatever the launch.
+// out[k] = the sum of line[d] over the distances in bucket k, by a workgroup of THREADS (line in LDS, complete; `ids`: n ints of LDS, `tmp`: THREADS
+// floats).  Fixed order: every bucket is cut into the same slices whatever the launch.
 template <int THREADS>
-__device__ __forceinline__ void rb_line_to_buckets(const float* line, const int32_t* __restrict__ map, int n, int buckets, float* out, float* tmp) {
+__device__ __forceinline__ void rb_line_to_buckets(const float* line, const int32_t* __restrict__ map, int n, int buckets, float* out, int* ids, float* tmp) {
+    for (int d = threadIdx.x; d < n; d += THREADS) ids[d] = map[d];
+    __syncthreads();
     int p = 1;
     while (p < buckets && p < THREADS) p <<= 1;
     const int slice = threadIdx.x / p, slices = THREADS / p;
@@ -27,7 +29,8 @@ __device__ __forceinline__ void rb_line_to_buckets(const float* line, const int3
     for (int k0 = 0; k0 < buckets; k0 += p) {
         const int k = k0 + (threadIdx.x & (p - 1));
         float acc = 0.f;
-        for (int d = from; d < to; ++d) acc += map[d] == k ? line[d] : 0.f;
+#pragma unroll 8
+        for (int d = from; d < to; ++d) acc += ids[d] == k ? line[d] : 0.f;
         __syncthreads();                               // (the last round's parts have been read)
         tmp[threadIdx.x] = acc;
         __syncthreads();

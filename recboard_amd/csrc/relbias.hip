@@ -50,6 +50,7 @@ template <class T, int VEC>
 __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
     constexpr int MAXD = (2 * RB_MAX_DISTANCE + 1 + 255) / 256;
     __shared__ float line[2 * RB_MAX_DISTANCE + 1];
+    __shared__ int ids[2 * RB_MAX_DISTANCE + 1];
     __shared__ float tmp[256];
     const int64_t h = blockIdx.y, i0 = (int64_t)blockIdx.x * RB_ROWS;
     const int R = a.R, band = 2 * R - 1;              // distances -(R - 1) .. R - 1
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
         line[2 * R] = tmp[4] + tmp[5] + tmp[6] + tmp[7];
     }
     __syncthreads();
-    rb_line_to_buckets<256>(line, a.map, 2 * R + 1, a.buckets, static_cast<float*>(a.out) + (h * gridDim.x + blockIdx.x) * a.buckets, tmp);
+    rb_line_to_buckets<256>(line, a.map, 2 * R + 1, a.buckets, static_cast<float*>(a.out) + (h * gridDim.x + blockIdx.x) * a.buckets, ids, tmp);
 }
 
 template <class T>
