@@ -31,7 +31,9 @@ static bwd_plan make_bwd_plan(const args& a, int dtype, bool vec, bool want_tabl
     const int chp = dtype == RE_F32 ? ch + 1 : ch <= 4 ? 4 : ch <= 8 ? 8 : 16;
     const size_t tiles = (size_t)4 * rows * chp * 16, n_line = 2 * a.R + 1;
     const size_t line = a.table ? line_len(a.R) * sizeof(float) : 0;
-    p.lds_q = tiles + line + (want_table ? p.wq * 2 * (n_line + 124) * sizeof(float) : 0);
+    // (the sums by distance; behind the loop a distance's bucket each and a float a lane)
+    const size_t by_wave = p.wq * (n_line + 124), by_lane = n_line + 64 * p.wq;
+    p.lds_q = tiles + line + (want_table ? (by_wave > by_lane ? by_wave : by_lane) * sizeof(float) : 0);
     p.lds_k = (size_t)(4 * qrows + (v_lds ? 32 * p.wk : 0)) * chp * 16 + 6 * qrows * sizeof(float) + line;
     return p;
 }
