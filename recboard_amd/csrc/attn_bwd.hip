@@ -86,7 +86,7 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
                                                                                               : attn::bwd_launch<re_f16>(a, io, p, st);
     if (r != RE_OK) return r;
     if (dtable)
-        hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)a.Hq), dim3(256), 0, st, io.part, (int64_t)a.B, (int64_t)a.Hq, p.qtiles * p.qsplits, a.buckets, dtable,
+        hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)a.Hq), dim3(1024), 0, st, io.part, (int64_t)a.B, (int64_t)a.Hq, p.qtiles * p.qsplits, a.buckets, dtable,
                            a.tdtype);
     return re_launch_status();
 }

@@ -53,3 +53,43 @@ __device__ __forceinline__ void re_store_vec(T* p, const float* f) {
     for (int i = 0; i < VEC; ++i) v.e[i] = (T)f[i];
     *reinterpret_cast<re_vec<T, VEC>*>(p) = v;
 }
+
+// VEC consecutive elements that start on any element (the hardware takes the address as it is), as far as they lie below `left` elements
+template <class T, int VEC, bool ALIGNED>
+__device__ __forceinline__ void re_load_some(const T* p, int left, float* f) {
+    if constexpr (ALIGNED) {
+        re_load_vec<T, VEC>(p, f);
+    } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) any {
+            T e[VEC];
+        };
+        if (left >= VEC) {
+            const any v = *reinterpret_cast<const any*>(p);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = (float)v.e[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) f[i] = i < left ? (float)p[i] : 0.f;
+        }
+    }
+}
+template <class T, int VEC, bool ALIGNED>
+__device__ __forceinline__ void re_store_some(T* p, int left, const float* f) {
+    if constexpr (ALIGNED) {
+        re_store_vec<T, VEC>(p, f);
+    } else {
+        struct __attribute__((packed, aligned(sizeof(T)))) any {
+            T e[VEC];
+        };
+        if (left >= VEC) {
+            any v;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v.e[i] = (T)f[i];
+            *reinterpret_cast<any*>(p) = v;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (i < left) p[i] = (T)f[i];
+        }
+    }
+}

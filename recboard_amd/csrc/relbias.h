@@ -41,17 +41,18 @@ __device__ __forceinline__ void rb_line_to_buckets(const float* line, const int3
     }
 }
 
-// dtable[k, h] = sum over r < rows of part[b][h][r][k] (b < B): one workgroup per head, 256 lanes = bucket x slice, fixed order
-static __global__ __launch_bounds__(256) void rb_reduce_k(const float* __restrict__ part, int64_t B, int64_t H, int64_t rows, int buckets, void* dtable,
-                                                          int32_t dtype) {
-    __shared__ float tmp[256];
+// dtable[k, h] = sum over r < rows of part[b][h][r][k] (b < B): one workgroup per head, 1024 lanes = bucket x slice (a few loads in flight each:
+// the launch is their latency), fixed order
+static __global__ __launch_bounds__(1024) void rb_reduce_k(const float* __restrict__ part, int64_t B, int64_t H, int64_t rows, int buckets, void* dtable,
+                                                           int32_t dtype) {
+    __shared__ float tmp[1024];
     int p = 1;
     while (p < buckets) p <<= 1;
-    const int k = threadIdx.x & (p - 1), slice = threadIdx.x / p, slices = 256 / p;
+    const int k = threadIdx.x & (p - 1), slice = threadIdx.x / p, slices = 1024 / p;
     const int64_t h = blockIdx.x, n = B * rows;
     float acc = 0.f;
     if (k < buckets) {
-#pragma unroll 4
+#pragma unroll 8
         for (int64_t i = slice; i < n; i += slices) {
             const int64_t b = i / rows, r = i - b * rows;
             acc += part[((b * H + h) * rows + r) * buckets + k];

@@ -11,7 +11,7 @@
 
 namespace {
 
-constexpr int RB_ROWS = 16;       // query rows of a workgroup
+constexpr int RB_ROWS = 16;       // query rows of a workgroup: every gridDim.x-th, so that the workgroups together walk through memory in order
 
 struct rb_args {
     const void* in;               // table / dbias
@@ -24,17 +24,17 @@ struct rb_args {
 template <class T, int VEC>
 __global__ __launch_bounds__(256) void rb_fwd_k(const rb_args a) {
     __shared__ T line[2 * RB_MAX_DISTANCE + 1];
-    const int64_t h = blockIdx.y, i0 = (int64_t)blockIdx.x * RB_ROWS;
+    const int64_t h = blockIdx.y;
     for (int d = threadIdx.x; d < 2 * a.R + 1; d += 256) {
         const int k = a.map[d];
         line[d] = (unsigned)k < (unsigned)a.buckets ? static_cast<const T*>(a.in)[k * a.H + h] : (T)0.f;
     }
     __syncthreads();
     const int64_t nv = (a.Sk + VEC - 1) / VEC;
-    const int rows = (int)min((int64_t)RB_ROWS, a.Sq - i0);
+    const int64_t rows = (a.Sq - blockIdx.x + gridDim.x - 1) / gridDim.x;
     // lanes run over (row, piece): short rows share a pass
     for (int64_t t = threadIdx.x; t < rows * nv; t += 256) {
-        const int64_t row = t / nv, j = (t - row * nv) * VEC, i = i0 + row;
+        const int64_t row = t / nv, j = (t - row * nv) * VEC, i = blockIdx.x + row * gridDim.x;
         const int64_t base = j - i - a.offset;
         re_vec<T, VEC> v;
 #pragma unroll
@@ -52,34 +52,63 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
     __shared__ float line[2 * RB_MAX_DISTANCE + 1];
     __shared__ int ids[2 * RB_MAX_DISTANCE + 1];
     __shared__ float tmp[256];
-    const int64_t h = blockIdx.y, i0 = (int64_t)blockIdx.x * RB_ROWS;
+    const int64_t h = blockIdx.y;
     const int R = a.R, band = 2 * R - 1;              // distances -(R - 1) .. R - 1
     float acc[MAXD];
 #pragma unroll
     for (int m = 0; m < MAXD; ++m) acc[m] = 0.f;
     float left = 0.f, right = 0.f;
-    const int64_t nv = a.Sk / VEC;                    // (VEC > 1 only where it divides Sk)
-    const int64_t i1 = min(i0 + RB_ROWS, a.Sq);
-    for (int64_t i = i0; i < i1; ++i) {
-        const T* g = static_cast<const T*>(a.in) + (h * a.Sq + i) * a.Sk;
-        const int64_t lo = i + a.offset - R, hi = i + a.offset + R;      // columns <= lo and >= hi are clipped
-        for (int64_t t = threadIdx.x; t < nv; t += 256) {
-            const int64_t j = t * VEC;
-            if (j > lo && j + VEC - 1 < hi) continue;
-            float f[VEC];
-            re_load_vec<T, VEC>(g + j, f);
+    // beyond the clipping distance: UR rows' pieces in flight at a time
+    constexpr int UR = 4;
+    const int64_t step = gridDim.x;
+    const int Sk = (int)a.Sk;
+    for (int64_t i = blockIdx.x; i < a.Sq; i += UR * step) {
+        const T* at[UR];                                 // (a row behind the last: the last, with nothing clipped)
+        int lo[UR], hi[UR];                              // row u: columns below lo and from hi on are clipped
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) {
-                left += j + e <= lo ? f[e] : 0.f;
-                right += j + e >= hi ? f[e] : 0.f;
+        for (int u = 0; u < UR; ++u) {
+            const int64_t l = i + u * step + a.offset - R + 1, r = i + u * step + a.offset + R;
+            const bool live = i + u * step < a.Sq;
+            at[u] = static_cast<const T*>(a.in) + (h * a.Sq + (live ? i + u * step : a.Sq - 1)) * a.Sk;
+            lo[u] = !live || l < 0 ? 0 : l > Sk ? Sk : (int)l;
+            hi[u] = !live || r > Sk ? Sk : r < 0 ? 0 : (int)r;
+        }
+        for (int j = threadIdx.x * VEC; j < Sk; j += 256 * VEC) {
+            float f[UR][VEC];
+            re_vec<T, VEC> v[UR];
+#pragma unroll
+            for (int u = 0; u < UR; ++u) v[u] = *reinterpret_cast<const re_vec<T, VEC>*>(at[u] + j);      // (no condition: all at once)
+#pragma unroll
+            for (int u = 0; u < UR; ++u)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) f[u][e] = (float)v[u].e[e];
+#pragma unroll
+            for (int u = 0; u < UR; ++u) {
+                if (j + VEC <= lo[u] || j >= hi[u]) {
+                    float sum = 0.f;
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) sum += f[u][e];
+                    left += j < lo[u] ? sum : 0.f;
+                    right += j < lo[u] ? 0.f : sum;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < VEC; ++e) {
+                        left += j + e < lo[u] ? f[u][e] : 0.f;
+                        right += j + e >= hi[u] ? f[u][e] : 0.f;
+                    }
+                }
             }
         }
+    }
+    // the band: lane d has distance d - (R - 1) of every row
 #pragma unroll
-        for (int m = 0; m < MAXD; ++m) {
-            if (m * 256 >= band) break;
-            const int d = m * 256 + threadIdx.x;
-            const int64_t j = lo + 1 + d;
-            if (d < band && j >= 0 && j < a.Sk) acc[m] += (float)g[j];
+    for (int m = 0; m < MAXD; ++m) {
+        if (m * 256 >= band) break;
+        const int d = m * 256 + threadIdx.x;
+#pragma unroll
+        for (int u = 0; u < RB_ROWS; ++u) {
+            const int64_t i = blockIdx.x + u * step, j = i + a.offset - R + 1 + d;
+            if (d < band && i < a.Sq && j >= 0 && j < a.Sk) acc[m] += (float)static_cast<const T*>(a.in)[(h * a.Sq + i) * a.Sk + j];
         }
     }
 #pragma unroll
@@ -158,7 +187,7 @@ extern "C" int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map
         const rb_args a{dbias, ws, bucket_map, H, Sq, Sk, rb_clip(offset), (int32_t)max_distance, (int32_t)buckets};
         rb_dispatch(true, a, dtype, dbias, st);
     }
-    hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)H), dim3(256), 0, st, (const float*)ws, (int64_t)1, H, any ? re_cdiv(Sq, RB_ROWS) : 0,
+    hipLaunchKernelGGL(rb_reduce_k, dim3((unsigned)H), dim3(1024), 0, st, (const float*)ws, (int64_t)1, H, any ? re_cdiv(Sq, RB_ROWS) : 0,
                        (int)buckets, dtable, table_dtype);
     return re_launch_status();
 }

@@ -1548,10 +1548,12 @@ def _a(t):
 def _call(device, fn, what, *args):
     """fn(*args, stream) on the current stream of the tensors' device, whichever device is current."""
     if device.index == torch.cuda.current_device():
-        lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+        code = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
-            lib.check(fn(*args, torch.cuda.current_stream(device).cuda_stream), what)
+            code = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if code:
+        lib.check(code, what)
 
 
 def _norm_params(x, weight, bias):
