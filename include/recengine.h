@@ -776,14 +776,17 @@ typedef struct re_attention {
     int32_t dtype, causal, mask_kind, table_dtype, reserved;
 } re_attention;
 
-/* out: strides `out_stride` (batch, head, row), stats [2, B, Hq, Sq] contiguous.  Few rows against many keys (one new token per sequence) are
+/* out: strides `out_stride` (batch, head, row), stats [2, B, Hq, Sq] contiguous.  out_low (bf16, fp16; 16-byte aligned, may be NULL)
+ * [B, Hq, Sq, (D + 7) / 8 * 8]: what rounding took from out, in its type, for a backward pass whose row sums of dout * out are then as
+ * exact as the scores.  Few rows against many keys (one new token per sequence) are
  * split over the keys and joined: the workspace holds the parts (0 bytes where nothing is split). */
 size_t re_attention_fwd_workspace_bytes(const re_attention* a);
-int re_attention_fwd(const re_attention* a, void* out, const int64_t* out_stride, float* stats, void* ws, size_t ws_bytes, re_stream_t stream);
-/* Its backward: q, k, v, ... as in the forward call, its out and stats, and dout (strides `dout_stride`).  dq, dk, dv: the inputs' type, any
+int re_attention_fwd(const re_attention* a, void* out, const int64_t* out_stride, float* stats, void* out_low, void* ws, size_t ws_bytes,
+                     re_stream_t stream);
+/* Its backward: q, k, v, ... as in the forward call, its out, stats and out_low (or NULL), and dout (strides `dout_stride`).  dq, dk, dv: the inputs' type, any
  * strides, every row written (rows of keys that no row sees: 0).  dtable [buckets, Hq] of type table_dtype, or NULL. */
 size_t re_attention_bwd_workspace_bytes(const re_attention* a);
-int re_attention_bwd(const re_attention* a, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
+int re_attention_bwd(const re_attention* a, const void* out, const int64_t* out_stride, const float* stats, const void* out_low, const void* dout,
                      const int64_t* dout_stride, void* dq, const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,
                      const int64_t* dv_stride, void* dtable, void* ws, size_t ws_bytes, re_stream_t stream);
 

@@ -5,7 +5,7 @@
 namespace attn {
 
 struct bwd_io {
-    const void *o, *dout;
+    const void *o, *low, *dout;    // low: what rounding took from o (attn_common.h); null: nothing is known of it
     void *dq, *dk, *dv;
     int64_t os[3], dos[3], dqs[3], dks[3], dvs[3];
     const float* stats;            // the forward's [max, log sum][B][Hq][Sq]

@@ -55,13 +55,13 @@ extern "C" size_t re_attention_bwd_workspace_bytes(const re_attention* d) {
     return attn::delta_bytes(a) + attn::kv_bytes(a, p) + attn::q_bytes(a, p) + (a.table ? attn::part_bytes(a, p) : 0);
 }
 
-extern "C" int re_attention_bwd(const re_attention* d, const void* out, const int64_t* out_stride, const float* stats, const void* dout,
+extern "C" int re_attention_bwd(const re_attention* d, const void* out, const int64_t* out_stride, const float* stats, const void* out_low, const void* dout,
                                 const int64_t* dout_stride, void* dq, const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,
                                 const int64_t* dv_stride, void* dtable, void* ws, size_t ws_bytes, re_stream_t stream) {
     attn::args a;
     const int rc = attn_args(d, a);
     if (rc != RE_OK) return rc;
-    if (!out_stride || !dout_stride || !dq_stride || !dk_stride || !dv_stride || (dtable && !a.table)) return RE_EINVAL;
+    if ((reinterpret_cast<uintptr_t>(out_low) & 15) || !out_stride || !dout_stride || !dq_stride || !dk_stride || !dv_stride || (dtable && !a.table)) return RE_EINVAL;
     if (attn_empty(a)) return a.B && a.Hq && a.Sk ? RE_EUNSUPPORTED : RE_OK;      // (no query, but gradients of keys to write: the caller's zeros)
     if (!a.q || !out || !stats || !dout || !dq || (a.Sk > 0 && (!a.k || !a.v || !dk || !dv))) return RE_EINVAL;
     const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}, {dout, dout_stride}, {dq, dq_stride},
@@ -71,7 +71,7 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
     const size_t kv = attn::kv_bytes(a, p), qb = attn::q_bytes(a, p), need = attn::delta_bytes(a) + kv + qb + (dtable ? attn::part_bytes(a, p) : 0);
     if (!ws || ws_bytes < need) return RE_EWORKSPACE;
     char* at = (char*)ws + attn::delta_bytes(a);
-    attn::bwd_io io{out, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, kv ? (float*)at : nullptr, p.splits, qb ? (float*)(at + kv) : nullptr,
+    attn::bwd_io io{out, d->dtype == RE_F32 ? nullptr : out_low, dout, dq, dk, dv, {}, {}, {}, {}, {}, stats, (float*)ws, kv ? (float*)at : nullptr, p.splits, qb ? (float*)(at + kv) : nullptr,
                     p.qsplits, dtable ? (float*)(at + kv + qb) : nullptr};
     for (int x = 0; x < 3; ++x) {
         io.os[x] = out_stride[x];

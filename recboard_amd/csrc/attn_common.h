@@ -239,6 +239,14 @@ __device__ __forceinline__ void place(const order& o, int id, int& unit, int& ti
     unit = (l / o.chunk * o.xcd + x) * o.chunk + l % o.chunk;
 }
 
+// What rounding took from a 16-bit output, in that type, for the backward's delta = rowsum(dO O): a row's probabilities sum to one, so an error of delta
+// is common to the whole row of dS, and in sums over it (a bias's gradient) it does not average out.  Rows of low_len(D) elements.
+__host__ __device__ inline int low_len(int D) { return (D + 7) / 8 * 8; }
+template <class T>
+__device__ __forceinline__ T* low_row(const args& a, void* low, int b, int h, int i) {
+    return static_cast<T*>(low) + (((int64_t)b * a.Hq + h) * a.Sq + i) * low_len(a.D);
+}
+
 // ---------------------------------------------------------------------------------------------------------- lengths, masks, bias
 __device__ __forceinline__ int seq_len(const args& a, int b) {
     if (!a.lens) return a.Sk;

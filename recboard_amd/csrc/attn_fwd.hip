@@ -44,19 +44,19 @@ extern "C" size_t re_attention_fwd_workspace_bytes(const re_attention* d) {
     return attn::make_plan(a, d->dtype, false).part;
 }
 
-extern "C" int re_attention_fwd(const re_attention* d, void* out, const int64_t* out_stride, float* stats, void* ws, size_t ws_bytes,
+extern "C" int re_attention_fwd(const re_attention* d, void* out, const int64_t* out_stride, float* stats, void* out_low, void* ws, size_t ws_bytes,
                                 re_stream_t stream) {
     attn::args a;
     const int rc = attn_args(d, a);
     if (rc != RE_OK) return rc;
-    if (!out_stride) return RE_EINVAL;
+    if (!out_stride || (reinterpret_cast<uintptr_t>(out_low) & 15)) return RE_EINVAL;
     if (attn_empty(a)) return RE_OK;
     if (!a.q || !out || !stats || (a.Sk > 0 && (!a.k || !a.v))) return RE_EINVAL;
     const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}});
     const attn::fwd_plan p = attn::make_plan(a, d->dtype, vec);
     if ((int64_t)a.B * p.heads * p.tiles * p.splits >= (1ll << 23)) return RE_EUNSUPPORTED;
     if (p.part && (!ws || ws_bytes < p.part)) return RE_EWORKSPACE;
-    const attn::fwd_out f{out, {out_stride[0], out_stride[1], out_stride[2]}, stats, p.part ? (float*)ws : nullptr,
+    const attn::fwd_out f{out, {out_stride[0], out_stride[1], out_stride[2]}, stats, d->dtype == RE_F32 ? nullptr : out_low, p.part ? (float*)ws : nullptr,
                           attn_order((int64_t)a.B * p.heads, (int64_t)p.tiles * p.splits, p.pg > 1 ? 1 : a.group), p.splits, p.tiles, p.heads, p.pg};
     re_clear_error();
     hipStream_t st = (hipStream_t)stream;

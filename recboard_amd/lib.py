@@ -137,9 +137,9 @@ SIGNATURES = {
     "re_relative_bias_bwd_workspace_bytes": (_sz, [_i64, _i64, _i64]),
     "re_relative_bias_bwd": (_i32, [_vp, _vp, _i64, _i64, _i64, _i64, _i64, _i64, _i32, _vp, _i32, _vp, _sz, _vp]),
     "re_attention_fwd_workspace_bytes": (_sz, [_vp]),
-    "re_attention_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "re_attention_fwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "re_attention_bwd_workspace_bytes": (_sz, [_vp]),
-    "re_attention_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "re_attention_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
 }
 
 _LIB = None

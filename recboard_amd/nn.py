@@ -167,7 +167,7 @@ def attention(q, k, v, *, scale=None, causal=False, mask=None, key_lengths=None,
     at = torch.is_tensor(q_offset)
     return _R.attention(q, k, v, 0.0 if scale is None else _positive(scale), bool(causal), mask, key_lengths, q_offset if at else None,
                         0 if at else k.shape[2] - q.shape[2] if q_offset is None else int(q_offset), None if position is None else position.weight,
-                        None if position is None else position.bucket_map)[0]
+                        None if position is None else position.bucket_map, torch.is_grad_enabled())[0]
 
 
 def _positive(scale):

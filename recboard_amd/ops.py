@@ -1770,7 +1770,19 @@ def _heads_of(B, S, H, D, like):
     return torch.empty_strided((B, H, S, D), (S * H * D, D, H * D, 1), dtype=like.dtype, device=like.device)
 
 
-def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, rel_table=None, bucket_map=None):
+def attention_planes(q):
+    """Planes of attention_fwd's stats: two; for a 16-bit type two more unused ones (the rest then starts on 16 bytes) and (D + 7) / 8 * 4 that hold a
+    row of D elements of it."""
+    return 2 if q.dtype == torch.float32 else 4 + (q.shape[3] + 7) // 8 * 4
+
+
+def _low_of(stats):
+    """The address of what lies behind the first four planes, or None."""
+    return None if stats.shape[0] == 2 else stats.data_ptr() + 16 * stats[0].numel()
+
+
+def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None, q_offset=None, rel_table=None, bucket_map=None,
+                  need_backward=True):
     """softmax(scale q k^T + bias + mask) v over the keys that a row may see (re_attention_fwd): q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], fp32,
     bf16 or fp16, any strides but adjacent elements in a row, D <= 128; Hkv a divisor of Hq (shared key heads).
 
@@ -1782,18 +1794,19 @@ def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None
                       key_lengths of a cache: key_lengths - Sq.
         rel_table, bucket_map   the relative position bias (relative_bias_fwd), made inside: table [buckets, Hq]
 
-    -> (out [B, Hq, Sq, D] laid out as [B, Sq, Hq, D], stats [2, B, Hq, Sq] fp32: the largest score of a row and the log of its sum, which add
-    up to the log of the softmax's denominator).  A row that sees no key: out 0, stats -inf and 0."""
+    -> (out [B, Hq, Sq, D] laid out as [B, Sq, Hq, D], stats [n, B, Hq, Sq] fp32).  stats[0], stats[1]: the largest score of a row and the log of its
+    sum, which add up to the log of the softmax's denominator; with bf16 / fp16 and need_backward, the planes behind them hold what rounding
+    took from out, for attention_bwd.  A row that sees no key: out 0, stats -inf and 0."""
     d = _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_table, bucket_map)
     B, Hq, Sq, D = q.shape
     out = _heads_of(B, Sq, Hq, D, q)
-    stats = torch.empty((2, B, Hq, Sq), dtype=torch.float32, device=q.device)
+    stats = torch.empty((attention_planes(q) if need_backward else 2, B, Hq, Sq), dtype=torch.float32, device=q.device)
     L = lib.load()
     p = ctypes.addressof(d)
     n = L.re_attention_fwd_workspace_bytes(p)
     ws = _ws(n, q.device) if n else None
     st = out.stride()
-    _call(q.device, L.re_attention_fwd, "re_attention_fwd", p, _a(out), _STRIDE3(st[0], st[1], st[2]), _a(stats), _a(ws), n)
+    _call(q.device, L.re_attention_fwd, "re_attention_fwd", p, _a(out), _STRIDE3(st[0], st[1], st[2]), _a(stats), _low_of(stats), _a(ws), n)
     return out, stats
 
 
@@ -1805,8 +1818,8 @@ def attention_bwd(dout, q, k, v, out, stats, scale=None, causal=False, mask=None
     Hkv, Sk = k.shape[1], k.shape[2]
     o_st, g_st = _rows4(out, "out", q)[1], _rows4(dout, "dout", q)[1]
     _req_any(stats, "stats", q.device, torch.float32)
-    if out.shape != q.shape or dout.shape != q.shape or stats.shape != (2, B, Hq, Sq):
-        raise ValueError("recengine: `out` and `dout` must have q's shape, `stats` [2, batch, heads, rows]")
+    if out.shape != q.shape or dout.shape != q.shape or stats.shape not in ((2, B, Hq, Sq), (attention_planes(q), B, Hq, Sq)):
+        raise ValueError("recengine: `out` and `dout` must have q's shape, `stats` [planes, batch, heads, rows]")
     dtable = None if rel_table is None else torch.empty_like(rel_table)
     dq, dk, dv = _heads_of(B, Sq, Hq, D, q), _heads_of(B, Sk, Hkv, D, q), _heads_of(B, Sk, Hkv, D, q)
     if not q.numel():                     # no row: nothing reaches the keys
@@ -1816,6 +1829,6 @@ def attention_bwd(dout, q, k, v, out, stats, scale=None, causal=False, mask=None
     L = lib.load()
     p = ctypes.addressof(d)
     ws = _ws(L.re_attention_bwd_workspace_bytes(p), q.device)
-    _call(q.device, L.re_attention_bwd, "re_attention_bwd", p, _a(out), o_st, _a(stats), _a(dout), g_st, _a(dq), _STRIDE3(*dq.stride()[:3]), _a(dk),
+    _call(q.device, L.re_attention_bwd, "re_attention_bwd", p, _a(out), o_st, _a(stats), _low_of(stats), _a(dout), g_st, _a(dq), _STRIDE3(*dq.stride()[:3]), _a(dk),
           _STRIDE3(*dk.stride()[:3]), _a(dv), _STRIDE3(*dv.stride()[:3]), _a(dtable), _a(ws), ws.numel())
     return dq, dk, dv, dtable

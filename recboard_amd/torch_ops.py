@@ -513,9 +513,10 @@ def _rows(t):
 @_lib.custom_op("recengine::attention", mutates_args=(), device_types="cuda")
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, causal: bool, mask: Optional[torch.Tensor],
               key_lengths: Optional[torch.Tensor], q_offsets: Optional[torch.Tensor], q_offset: int, table: Optional[torch.Tensor],
-              bucket_map: Optional[torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+              bucket_map: Optional[torch.Tensor], need_backward: bool = True) -> tuple[torch.Tensor, torch.Tensor]:
     return ops.attention_fwd(_rows(q), _rows(k), _rows(v), scale=scale or None, causal=causal, mask=mask, key_lengths=key_lengths,
-                             q_offset=q_offset if q_offsets is None else q_offsets, rel_table=_c(table), bucket_map=bucket_map)
+                             q_offset=q_offset if q_offsets is None else q_offsets, rel_table=_c(table), bucket_map=bucket_map,
+                             need_backward=need_backward)
 
 
 def _heads_like(t):
@@ -524,8 +525,8 @@ def _heads_like(t):
 
 
 @attention.register_fake
-def _(q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map):
-    return _heads_like(q), q.new_empty((2,) + tuple(q.shape[:3]), dtype=torch.float32)
+def _(q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map, need_backward=True):
+    return _heads_like(q), q.new_empty((ops.attention_planes(q) if need_backward else 2,) + tuple(q.shape[:3]), dtype=torch.float32)
 
 
 @_lib.custom_op("recengine::attention_backward", mutates_args=(), device_types="cuda")
@@ -544,7 +545,7 @@ def _(dout, q, k, v, out, stats, scale, causal, mask, key_lengths, q_offsets, q_
 
 
 def _attn_setup(ctx, inputs, output):
-    q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map = inputs
+    q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map, need_backward = inputs
     ctx.set_materialize_grads(False)
     ctx.save_for_backward(q, k, v, output[0], output[1], mask, key_lengths, q_offsets, table, bucket_map)
     ctx.scale, ctx.causal, ctx.q_offset = scale, causal, q_offset
@@ -552,11 +553,11 @@ def _attn_setup(ctx, inputs, output):
 
 def _attn_bwd(ctx, dout, dstats):
     if dout is None:
-        return (None,) * 11
+        return (None,) * 12
     q, k, v, out, stats, mask, key_lengths, q_offsets, table, bucket_map = ctx.saved_tensors
     g = torch.ops.recengine.attention_backward(dout, q, k, v, out, stats, ctx.scale, ctx.causal, mask, key_lengths, q_offsets, ctx.q_offset, table,
                                                bucket_map)
-    return g[0], g[1], g[2], None, None, None, None, None, None, g[3] if table is not None else None, None
+    return g[0], g[1], g[2], None, None, None, None, None, None, g[3] if table is not None else None, None, None
 
 
 attention.register_autograd(_attn_bwd, setup_context=_attn_setup)

@@ -22,14 +22,14 @@ def desc(**kw):
     return d
 
 
-def fwd(d, out=P, stats=P, ws=P, n=1 << 40):
+def fwd(d, out=P, stats=P, ws=P, n=1 << 40, low=None):
     st = (ctypes.c_int64 * 3)(51200, 64, 512)
-    return lib.load().re_attention_fwd(ctypes.addressof(d), out, st, stats, ws, n, None)
+    return lib.load().re_attention_fwd(ctypes.addressof(d), out, st, stats, low, ws, n, None)
 
 
 def bwd(d, n=1 << 40, dtable=None):
     st = (ctypes.c_int64 * 3)(51200, 64, 512)
-    return lib.load().re_attention_bwd(ctypes.addressof(d), P, st, P, P, st, P, st, P, st, P, st, dtable, P, n, None)
+    return lib.load().re_attention_bwd(ctypes.addressof(d), P, st, P, None, P, st, P, st, P, st, P, st, dtable, P, n, None)
 
 
 @pytest.mark.parametrize("bad,code", [({"D": 0}, EINVAL), ({"D": 129}, EUNSUPPORTED), ({"Hkv": 3}, EINVAL), ({"Hkv": 0}, EINVAL), ({"B": -1}, EINVAL), ({"dtype": 3}, EINVAL),
@@ -46,7 +46,8 @@ def test_attention_refuses_what_it_cannot_do(bad, code):
 def test_attention_refuses_missing_outputs_and_short_workspaces():
     L = lib.load()
     assert fwd(desc(), out=None) == EINVAL and fwd(desc(), stats=None) == EINVAL
-    assert L.re_attention_fwd(None, P, None, P, P, 0, None) == EINVAL
+    assert L.re_attention_fwd(None, P, None, P, None, P, 0, None) == EINVAL
+    assert fwd(desc(), low=ctypes.c_void_p(4104)) == EINVAL
     one = desc(Sq=1, Sk=16384)
     need = L.re_attention_fwd_workspace_bytes(ctypes.addressof(one))
     assert need > 0 and fwd(one, n=need - 1) == EWORKSPACE and fwd(one, ws=None) == EWORKSPACE

@@ -72,8 +72,8 @@ def reference(q, k, v, scale=None, causal=False, mask=None, key_lengths=None, q_
     dp = g @ vT
     delta = (p * dp).sum(3, keepdim=True)
     ds = p * (dp - delta)
-    # delta comes from the rounded output: dO . (out + its error)
-    e_delta = (g.abs() * out_tol).sum(3, keepdim=True) + D * F * (g.abs() * out.abs()).sum(3, keepdim=True)
+    # delta comes from the output and what rounding took from it (u^2 is left): dO . (out + its error before rounding)
+    e_delta = (g.abs() * (out_tol - u * out.abs() * (1 - u))).sum(3, keepdim=True) + D * F * (g.abs() * out.abs()).sum(3, keepdim=True)
     e_dp = (D + 4) * F * (g.abs() @ vT.abs())
     dse = pe * (dp - delta).abs() + (p + pe) * (e_dp + e_delta)
     mag_s = ds.abs() + dse
@@ -108,7 +108,10 @@ def check(q, k, v, dout=None, **how):
     out, stats = ops.attention_fwd(q, k, v, **how)
     want = reference(q, k, v, dout=dout, **how)
     compare(out, want["out"], "out")
-    lse = stats.sum(0)
+    lse = stats[0] + stats[1]
+    lean, two = ops.attention_fwd(q, k, v, need_backward=False, **how)
+    assert torch.equal(lean, out) or not torch.isfinite(out).all()
+    assert two.shape[0] == 2 and torch.equal(two, stats[:2])
     compare(lse, want["lse"], "lse")
     if dout is None:
         return out, lse
@@ -296,6 +299,31 @@ def test_attention_of_nothing():
     assert not dk.any() and not dv.any()
     out, lse = ops.attention_fwd(q[:0], k[:0], v[:0])
     assert out.shape == (0, 4, 5, 32)
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+def test_attention_position_gradient_is_as_exact_as_the_scores(t):
+    """The rows of dS sum to zero, so an error of delta does not average out of the bias's gradient: with delta from the rounded output it was 2^-9 of
+    |dO| |out| per row.  What is left is the scores' fp32 error and the rounding of P in the output, n * u / sqrt(n) of its terms at random: within
+    1.5 roundings of the result in the 2-norm."""
+    from recboard_amd import ops
+    q, k, v, dout = make(2, 4, 4, 512, 512, 64, t)
+    how = rel(4, t)
+    out, stats = ops.attention_fwd(q, k, v, **how)
+    got = ops.attention_bwd(dout, q, k, v, out, stats, **how)[3].double()
+    want = reference(q, k, v, dout=dout, **how)["dtable"][0]
+    plain = ops.attention_bwd(dout, q, k, v, out, stats[:2].contiguous(), **how)[3].double()
+    near, far = ((x - want).norm() / want.norm() for x in (got, plain))
+    assert near < far and near <= 1.5 * torch.finfo(t).eps / 2, (float(near), float(far))
+
+
+@pytest.mark.parametrize("R", [24, 40, 100])
+def test_attention_with_the_position_bias_run_to_run(R):
+    q, k, v, _ = make(1, 4, 2, 150, 333, 64, torch.bfloat16)
+    from recboard_amd import ops
+    how = rel(4, torch.bfloat16, 16, R)
+    first = ops.attention_fwd(q, k, v, **how)[0]
+    assert all(torch.equal(first, ops.attention_fwd(q, k, v, **how)[0]) for _ in range(20))
 
 
 def test_attention_same_bits_again_on_another_stream_and_in_graphs():

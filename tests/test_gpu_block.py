@@ -171,7 +171,7 @@ def test_every_new_op_passes_opcheck_and_refuses_the_cpu():
     mask = torch.rand(2, 1, 1, 7, device="cuda") < 0.8
     torch.library.opcheck(R.attention.default, (q, k, v, 0.0, False, mask, None, None, 2, table, m), test_utils=tests)
     lens = torch.tensor([3, 7], device="cuda")
-    torch.library.opcheck(R.attention.default, (q, k, v, 0.3, True, None, lens, lens - 2, 0, None, None), test_utils=tests)
+    torch.library.opcheck(R.attention.default, (q, k, v, 0.3, True, None, lens, lens - 2, 0, None, None, True), test_utils=tests)
     for call in (lambda: R.layer_norm(x.cpu(), None, None), lambda: R.attention(q.cpu(), k.cpu(), v.cpu(), 0.0, False, None, None, None, 0, None, None),
                  lambda: R.relative_bias(table.cpu(), m.cpu(), 2, 2, 0)):
         with pytest.raises(RuntimeError):
