@@ -784,7 +784,8 @@ size_t re_attention_fwd_workspace_bytes(const re_attention* a);
 int re_attention_fwd(const re_attention* a, void* out, const int64_t* out_stride, float* stats, void* out_low, void* ws, size_t ws_bytes,
                      re_stream_t stream);
 /* Its backward: q, k, v, ... as in the forward call, its out, stats and out_low (or NULL), and dout (strides `dout_stride`).  dq, dk, dv: the inputs' type, any
- * strides, every row written (rows of keys that no row sees: 0).  dtable [buckets, Hq] of type table_dtype, or NULL. */
+ * strides, every row written (rows of keys that no row sees: 0).  dtable [buckets, Hq] of type table_dtype, or NULL.  Without any query row
+ * there is nothing to launch: RE_EUNSUPPORTED where a gradient would have to be written (zeros are the caller's). */
 size_t re_attention_bwd_workspace_bytes(const re_attention* a);
 int re_attention_bwd(const re_attention* a, const void* out, const int64_t* out_stride, const float* stats, const void* out_low, const void* dout,
                      const int64_t* dout_stride, void* dq, const int64_t* dq_stride, void* dk, const int64_t* dk_stride, void* dv,

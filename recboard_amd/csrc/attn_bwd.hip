@@ -62,7 +62,7 @@ extern "C" int re_attention_bwd(const re_attention* d, const void* out, const in
     const int rc = attn_args(d, a);
     if (rc != RE_OK) return rc;
     if ((reinterpret_cast<uintptr_t>(out_low) & 15) || !out_stride || !dout_stride || !dq_stride || !dk_stride || !dv_stride || (dtable && !a.table)) return RE_EINVAL;
-    if (attn_empty(a)) return a.B && a.Hq && a.Sk ? RE_EUNSUPPORTED : RE_OK;      // (no query, but gradients of keys to write: the caller's zeros)
+    if (attn_empty(a)) return (a.B && a.Hq && a.Sk) || (dtable && a.Hq) ? RE_EUNSUPPORTED : RE_OK;      // (no row, but gradients to write: the caller's zeros)
     if (!a.q || !out || !stats || !dout || !dq || (a.Sk > 0 && (!a.k || !a.v || !dk || !dv))) return RE_EINVAL;
     const bool vec = attn_aligned(a, d->dtype, {{a.q, a.qs}, {a.k, a.ks}, {a.v, a.vs}, {out, out_stride}, {dout, dout_stride}, {dq, dq_stride},
                                                 {dk, dk_stride}, {dv, dv_stride}});

@@ -4,7 +4,7 @@
 //   dtable[k, h]  = sum of dbias[h, i, j] over the pairs whose clipped distance lies in bucket k
 //
 // Bound by HBM: H Sq Sk elements written, or read, once.  Forward: the 2 R + 1 values of a head sit in LDS and a lane looks up the VEC elements of
-// one 16-byte store.  Backward: a lane owns DIAGONALS inside the band |j - i - offset| < R -- its column moves with the row, so the sum of a
+// one 16-byte store (rows may start anywhere).  Backward: a lane owns DIAGONALS inside the band |j - i - offset| < R -- its column moves with the row, so the sum of a
 // diagonal stays in one register -- while the two clipped sides (one bucket each) are summed with 16-byte loads.  A workgroup's diagonals are
 // then added into its buckets and the workgroups' buckets by a second launch, in a fixed order.
 #include "relbias.h"
@@ -21,7 +21,7 @@ struct rb_args {
     int32_t R, buckets;
 };
 
-template <class T, int VEC>
+template <class T, int VEC, bool ALIGNED>
 __global__ __launch_bounds__(256) void rb_fwd_k(const rb_args a) {
     __shared__ T line[2 * RB_MAX_DISTANCE + 1];
     const int64_t h = blockIdx.y;
@@ -36,17 +36,17 @@ __global__ __launch_bounds__(256) void rb_fwd_k(const rb_args a) {
     for (int64_t t = threadIdx.x; t < rows * nv; t += 256) {
         const int64_t row = t / nv, j = (t - row * nv) * VEC, i = blockIdx.x + row * gridDim.x;
         const int64_t base = j - i - a.offset;
-        re_vec<T, VEC> v;
+        float v[VEC];                                  // (exact: every type's values are floats)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) {
             const int64_t d = base + e;
-            v.e[e] = line[(d < -a.R ? -a.R : d > a.R ? a.R : (int)d) + a.R];
+            v[e] = (float)line[(d < -a.R ? -a.R : d > a.R ? a.R : (int)d) + a.R];
         }
-        *reinterpret_cast<re_vec<T, VEC>*>(static_cast<T*>(a.out) + (h * a.Sq + i) * a.Sk + j) = v;
+        re_store_some<T, VEC, ALIGNED>(static_cast<T*>(a.out) + (h * a.Sq + i) * a.Sk + j, (int)(a.Sk - j), v);
     }
 }
 
-template <class T, int VEC>
+template <class T, int VEC, bool ALIGNED>
 __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
     constexpr int MAXD = (2 * RB_MAX_DISTANCE + 1 + 255) / 256;
     __shared__ float line[2 * RB_MAX_DISTANCE + 1];
@@ -75,16 +75,11 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
         }
         for (int j = threadIdx.x * VEC; j < Sk; j += 256 * VEC) {
             float f[UR][VEC];
-            re_vec<T, VEC> v[UR];
 #pragma unroll
-            for (int u = 0; u < UR; ++u) v[u] = *reinterpret_cast<const re_vec<T, VEC>*>(at[u] + j);      // (no condition: all at once)
-#pragma unroll
-            for (int u = 0; u < UR; ++u)
-#pragma unroll
-                for (int e = 0; e < VEC; ++e) f[u][e] = (float)v[u].e[e];
+            for (int u = 0; u < UR; ++u) re_load_some<T, VEC, ALIGNED>(at[u] + j, Sk - j, f[u]);      // (whatever is clipped: all at once)
 #pragma unroll
             for (int u = 0; u < UR; ++u) {
-                if (j + VEC <= lo[u] || j >= hi[u]) {
+                if (j + VEC <= lo[u] || (j >= hi[u] && (ALIGNED || j + VEC <= Sk))) {
                     float sum = 0.f;
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) sum += f[u][e];
@@ -94,7 +89,7 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
 #pragma unroll
                     for (int e = 0; e < VEC; ++e) {
                         left += j + e < lo[u] ? f[u][e] : 0.f;
-                        right += j + e >= hi[u] ? f[u][e] : 0.f;
+                        right += j + e >= hi[u] && (ALIGNED || j + e < Sk) ? f[u][e] : 0.f;
                     }
                 }
             }
@@ -132,22 +127,22 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
 }
 
 template <class T>
-void rb_launch(bool bwd, const rb_args& a, bool vec, dim3 grid, hipStream_t st) {
+void rb_launch(bool bwd, const rb_args& a, bool aligned, dim3 grid, hipStream_t st) {
     constexpr int V = re_type<T>::VEC;
     if (bwd) {
-        if (vec) hipLaunchKernelGGL((rb_bwd_k<T, V>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rb_bwd_k<T, 1>), grid, dim3(256), 0, st, a);
+        if (aligned) hipLaunchKernelGGL((rb_bwd_k<T, V, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rb_bwd_k<T, V, false>), grid, dim3(256), 0, st, a);
     } else {
-        if (vec) hipLaunchKernelGGL((rb_fwd_k<T, V>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((rb_fwd_k<T, 1>), grid, dim3(256), 0, st, a);
+        if (aligned) hipLaunchKernelGGL((rb_fwd_k<T, V, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((rb_fwd_k<T, V, false>), grid, dim3(256), 0, st, a);
     }
 }
 int rb_dispatch(bool bwd, const rb_args& a, int32_t dtype, const void* big, hipStream_t st) {
-    const bool vec = a.Sk % (16 / (int64_t)re_dtype_size(dtype)) == 0 && (reinterpret_cast<uintptr_t>(big) & 15) == 0;
+    const bool aligned = a.Sk % (16 / (int64_t)re_dtype_size(dtype)) == 0 && (reinterpret_cast<uintptr_t>(big) & 15) == 0;
     const dim3 grid((unsigned)re_cdiv(a.Sq, RB_ROWS), (unsigned)a.H);
-    if (dtype == RE_F32) rb_launch<float>(bwd, a, vec, grid, st);
-    else if (dtype == RE_BF16) rb_launch<re_bf16>(bwd, a, vec, grid, st);
-    else rb_launch<re_f16>(bwd, a, vec, grid, st);
+    if (dtype == RE_F32) rb_launch<float>(bwd, a, aligned, grid, st);
+    else if (dtype == RE_BF16) rb_launch<re_bf16>(bwd, a, aligned, grid, st);
+    else rb_launch<re_f16>(bwd, a, aligned, grid, st);
     return 0;
 }
 bool rb_shape_ok(int64_t H, int64_t Sq, int64_t Sk) { return H >= 0 && Sq >= 0 && Sk >= 0 && H <= 65535 && Sq <= (1ll << 27) && Sk <= (1ll << 30); }

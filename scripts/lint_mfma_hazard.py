@@ -12,6 +12,7 @@ import re
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 # passes on gfx950.  The 16-bit forms CDNA3 already had run at CDNA3's rate there (1 307 TF dense on 304 CUs x 4 SIMDs x 2.1 GHz = 512 FLOP per
@@ -112,25 +113,34 @@ def lint_function(name, ins):
     return findings
 
 
+def no_packed(src):
+    """The files that the Makefile compiles without packed-fp32 instructions."""
+    name = os.path.basename(src)
+    return name in ("enc_tile.hip", "layernorm.hip", "relbias.hip") or name.startswith("attn_")
+
+
 def main():
     srcs = sys.argv[1:] or sorted(glob.glob(os.path.join(ROOT, "recboard_amd", "csrc", "*.hip")))
     bad = 0
     with tempfile.TemporaryDirectory() as td:
-        for src in srcs:
+        # the files are compiled side by side (the attention instances take a minute each), read one after the other
+        def compiled(src):
             out = os.path.join(td, os.path.basename(src) + ".s")
+            extra = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if no_packed(src) else []
+            subprocess.run(["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-S", "--cuda-device-only"] + extra + [
+                            "-I" + os.path.join(ROOT, "recboard_amd", "csrc"), "-I" + os.path.join(ROOT, "include"), src, "-o", out], check=True)
+            return out
+        with ThreadPoolExecutor(min(6, os.cpu_count() or 1)) as pool:
+            outs = list(pool.map(compiled, srcs))
+        for src, out in zip(srcs, outs):
             # enc_tile.hip is built WITHOUT packed-fp32 instructions (csrc/Makefile: TILE_FLAGS; profiles/r6_handover_notes.txt): the lint compiles it
             # as the product does and checks that none is left -- with them the tile kernels are not reproducible once two waves share a SIMD
-            tile = os.path.basename(src) == "enc_tile.hip"
-            extra = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] if tile else []
-            cmd = ["/opt/rocm/bin/hipcc", "-O3", "-std=c++17", "--offload-arch=gfx950", "-S", "--cuda-device-only"] + extra + [
-                   "-I" + os.path.join(ROOT, "recboard_amd", "csrc"), "-I" + os.path.join(ROOT, "include"), src, "-o", out]
-            subprocess.run(cmd, check=True)
-            if tile:
+            if no_packed(src):
                 n_pk = sum(1 for ln in open(out) if re.match(r"\s+v_pk_(mul|add|fma)_f32\b", ln))
                 print("%-24s %5d packed-fp32 instructions" % (os.path.basename(src), n_pk))
                 if n_pk:
                     bad += 1
-                    print("HAZARD enc_tile.hip: %d v_pk_*_f32 instructions (the Makefile's TILE_FLAGS must reach this file)" % n_pk)
+                    print("HAZARD %s: %d v_pk_*_f32 instructions (the Makefile's TILE_FLAGS must reach this file)" % (os.path.basename(src), n_pk))
             n_mfma = 0
             for fn, ins in parse(out).items():
                 n_mfma += sum(1 for _, m, _ in ins if m and m.startswith("v_mfma"))

@@ -326,10 +326,11 @@ def test_attention_with_the_position_bias_run_to_run(R):
     assert all(torch.equal(first, ops.attention_fwd(q, k, v, **how)[0]) for _ in range(20))
 
 
-def test_attention_same_bits_again_on_another_stream_and_in_graphs():
+@pytest.mark.parametrize("D", [64, 128])
+def test_attention_same_bits_again_on_another_stream_and_in_graphs(D):
     from recboard_amd import ops
     from recboard_amd.capture import recording
-    q, k, v, dout = make(2, 4, 2, 200, 200, 64, torch.bfloat16)
+    q, k, v, dout = make(2, 4, 2, 200, 200, D, torch.bfloat16)
     how = {"causal": True, **rel(4, torch.float32, 32, 64, False)}
     one = q[:, :, :1].contiguous()
 
