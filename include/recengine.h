@@ -749,8 +749,9 @@ int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t b
                          int64_t Sk, int64_t offset, int32_t dtype, void* dtable, int32_t table_dtype, void* ws, size_t ws_bytes,
                          re_stream_t stream);
 
-/* Attention:  out = softmax over the keys a row may see of (scale q k^T + bias + mask), times v;  stats = each row's largest score and the log
- * of its sum of exp(score - largest): their sum is the log of the softmax's denominator, and apart they serve rows of any magnitude.
+/* Attention:  out = softmax over the keys a row may see of (scale q k^T + bias + mask), times v;  stats = each row's reference score m (its
+ * largest, or at most 8 log 2 below it) and the log of its sum of exp(score - m): their sum is the log of the softmax's denominator, and apart
+ * they serve rows of any magnitude.
  * q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], Hkv a divisor of Hq (query head h reads key head h / (Hq / Hkv)), any batch / head / row
  * strides (in elements, 0 for a broadcast one), D adjacent elements in a row, 1 <= D <= 128.
  * The keys that query i of sequence b may see: j < key_lengths[b] (DEVICE int64 [B], optional; values outside [0, Sk] are clipped), with

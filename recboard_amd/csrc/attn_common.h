@@ -228,14 +228,14 @@ __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4
 // of them); and there `set` units run side by side, tile by tile, so that the long tiles of all of them start before the short ones of any
 // (2 x 16 heads x 4096 x 128, causal, forward: 238 us a head at a time, 185 so).
 struct order {
-    int32_t xcd, units, tiles, set, chunk;      // xcd: 8, or 1; units per XCD; set divides units
+    int32_t xcd, units, tiles, set, chunk;      // xcd: 8, or 1; units per XCD (the last set may be smaller)
 };
 __device__ __forceinline__ void place(const order& o, int id, int& unit, int& tile) {
     const int x = id % o.xcd;
     id /= o.xcd;
-    const int per = o.set * o.tiles, first = id / per * o.set, r = id % per;
-    tile = r / o.set;
-    const int l = first + r % o.set;
+    const int per = o.set * o.tiles, first = id / per * o.set, r = id % per, wide = min(o.set, o.units - first);
+    tile = r / wide;
+    const int l = first + r % wide;
     unit = (l / o.chunk * o.xcd + x) * o.chunk + l % o.chunk;
 }
 
@@ -407,10 +407,8 @@ static inline attn::order attn_order(int64_t units, int64_t tiles, int chunk) {
     o.units = (int32_t)(units / o.xcd);
     o.tiles = (int32_t)tiles;
     // a set fills an XCD's 32 units of two workgroups each twice over
-    int64_t set = re_cdiv(128 * (8 / o.xcd), tiles);
-    set = set < o.units ? set : o.units;
-    while (o.units % set) ++set;
-    o.set = (int32_t)set;
+    const int64_t set = re_cdiv(128 * (8 / o.xcd), tiles);
+    o.set = (int32_t)(set < o.units ? set : o.units);
     return o;
 }
 

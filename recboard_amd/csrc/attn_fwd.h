@@ -7,7 +7,7 @@ namespace attn {
 struct fwd_out {
     void* o;
     int64_t os[3];                 // batch, head, row
-    float* stats;                  // [max, log sum][B][Hq][Sq]
+    float* stats;                  // [reference score, log sum relative to it][B][Hq][Sq]
     void* low;                     // [B][Hq][Sq][low_len(D)]: what rounding took from o; null: not wanted
     float* part;                   // [splits][B][Hq][Sq][D], then [splits][B][Hq][Sq][2]; null: one split
     order ord;                     // units: workgroup heads of all sequences; tiles: query tiles x splits

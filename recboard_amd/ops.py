@@ -1794,8 +1794,8 @@ def attention_fwd(q, k, v, scale=None, causal=False, mask=None, key_lengths=None
                       key_lengths of a cache: key_lengths - Sq.
         rel_table, bucket_map   the relative position bias (relative_bias_fwd), made inside: table [buckets, Hq]
 
-    -> (out [B, Hq, Sq, D] laid out as [B, Sq, Hq, D], stats [n, B, Hq, Sq] fp32).  stats[0], stats[1]: the largest score of a row and the log of its
-    sum, which add up to the log of the softmax's denominator; with bf16 / fp16 and need_backward, the planes behind them hold what rounding
+    -> (out [B, Hq, Sq, D] laid out as [B, Sq, Hq, D], stats [n, B, Hq, Sq] fp32).  stats[0], stats[1]: a row's reference score (its largest, or at
+    most 8 log 2 below it) and the log of its sum relative to that, which add up to the log of the softmax's denominator; with bf16 / fp16 and need_backward, the planes behind them hold what rounding
     took from out, for attention_bwd.  A row that sees no key: out 0, stats -inf and 0."""
     d = _attention_args(q, k, v, scale, causal, mask, key_lengths, q_offset, rel_table, bucket_map)
     B, Hq, Sq, D = q.shape
