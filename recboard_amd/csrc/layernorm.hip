@@ -75,6 +75,35 @@ __device__ __forceinline__ void row_sum2(float& a, float& c, float* red) {
     }
 }
 
+// the lane's pieces of a weight (null: `none` everywhere; beyond D: 0).  Of the tensor's own type, the usual case, by 16-byte pieces; of another
+// element by element (a served token's row is its weights' latency: 7.8 us for one row of 4096 with the element loads, all types).
+template <class T, int LPR, int VEC, int N>
+__device__ __forceinline__ void load_weight(const void* w, int32_t wtype, int D, int lane, float none, float* f) {
+    if (!w) {
+#pragma unroll
+        for (int i = 0; i < N * VEC; ++i) f[i] = none;
+    } else if (wtype == re_type<T>::CODE) {
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            const int e = (n * LPR + lane) * VEC;
+            if (e < D) {
+                re_load_some<T, VEC, false>(static_cast<const T*>(w) + e, D - e, f + n * VEC);
+            } else {
+#pragma unroll
+                for (int v = 0; v < VEC; ++v) f[n * VEC + v] = 0.f;
+            }
+        }
+    } else {
+#pragma unroll
+        for (int n = 0; n < N; ++n)
+#pragma unroll
+            for (int v = 0; v < VEC; ++v) {
+                const int e = (n * LPR + lane) * VEC + v;
+                f[n * VEC + v] = e < D ? re_load_as_float(w, e, wtype) : 0.f;
+            }
+    }
+}
+
 template <class T, int LPR, int VEC, int N, bool ALIGNED>
 __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void ln_fwd_k(const ln_args a) {
     constexpr int THREADS = LPR > 256 ? LPR : 256, RPW = THREADS / LPR;
@@ -82,14 +111,8 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void ln_fwd_k(const ln_args 
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const int D = a.D;
     float w[N * VEC], b[N * VEC];
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int e = (n * LPR + lane) * VEC + v;
-            w[n * VEC + v] = a.w && e < D ? re_load_as_float(a.w, e, a.wtype) : 1.f;
-            b[n * VEC + v] = a.b && e < D ? re_load_as_float(a.b, e, a.wtype) : 0.f;
-        }
+    load_weight<T, LPR, VEC, N>(a.w, a.wtype, D, lane, 1.f, w);
+    load_weight<T, LPR, VEC, N>(a.b, a.wtype, D, lane, 0.f, b);
     const float inv_d = 1.f / (float)D;
     const int64_t steps = (a.rows + RPW - 1) / RPW;
     for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {
@@ -161,14 +184,9 @@ __global__ __launch_bounds__(LPR > 256 ? LPR : 256) void ln_bwd_k(const ln_bwd_a
     const int lane = threadIdx.x % LPR, sub = threadIdx.x / LPR;
     const int D = a.D;
     float w[N * VEC], dw[N * VEC], db[N * VEC];
+    load_weight<T, LPR, VEC, N>(a.w, a.wtype, D, lane, 1.f, w);
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-#pragma unroll
-        for (int v = 0; v < VEC; ++v) {
-            const int e = (n * LPR + lane) * VEC + v;
-            w[n * VEC + v] = a.w && e < D ? re_load_as_float(a.w, e, a.wtype) : 1.f;
-            dw[n * VEC + v] = db[n * VEC + v] = 0.f;
-        }
+    for (int i = 0; i < N * VEC; ++i) dw[i] = db[i] = 0.f;
     const float inv_d = 1.f / (float)D;
     const int64_t steps = (a.rows + RPW - 1) / RPW;
     for (int64_t step = blockIdx.x; step < steps; step += gridDim.x) {

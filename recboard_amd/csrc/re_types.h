@@ -14,14 +14,17 @@ template <class T>
 struct re_type;
 template <>
 struct re_type<float> {
+    static constexpr int32_t CODE = RE_F32;
     static constexpr int VEC = 4;      // elements of a 16-byte load
 };
 template <>
 struct re_type<re_bf16> {
+    static constexpr int32_t CODE = RE_BF16;
     static constexpr int VEC = 8;
 };
 template <>
 struct re_type<re_f16> {
+    static constexpr int32_t CODE = RE_F16;
     static constexpr int VEC = 8;
 };
 

@@ -65,6 +65,7 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
     for (int64_t i = blockIdx.x; i < a.Sq; i += UR * step) {
         const T* at[UR];                                 // (a row behind the last: the last, with nothing clipped)
         int lo[UR], hi[UR];                              // row u: columns below lo and from hi on are clipped
+        bool any = false;
 #pragma unroll
         for (int u = 0; u < UR; ++u) {
             const int64_t l = i + u * step + a.offset - R + 1, r = i + u * step + a.offset + R;
@@ -72,7 +73,9 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
             at[u] = static_cast<const T*>(a.in) + (h * a.Sq + (live ? i + u * step : a.Sq - 1)) * a.Sk;
             lo[u] = !live || l < 0 ? 0 : l > Sk ? Sk : (int)l;
             hi[u] = !live || r > Sk ? Sk : r < 0 ? 0 : (int)r;
+            any |= lo[u] > 0 || hi[u] < Sk;
         }
+        if (!any) continue;                              // (rows shorter than the clipping distance lie in the band)
         for (int j = threadIdx.x * VEC; j < Sk; j += 256 * VEC) {
             float f[UR][VEC];
 #pragma unroll
@@ -100,10 +103,16 @@ __global__ __launch_bounds__(256) void rb_bwd_k(const rb_args a) {
     for (int m = 0; m < MAXD; ++m) {
         if (m * 256 >= band) break;
         const int d = m * 256 + threadIdx.x;
+        float x[RB_ROWS];                                                // (clamped places, so that all rows' loads are in flight at once)
 #pragma unroll
         for (int u = 0; u < RB_ROWS; ++u) {
             const int64_t i = blockIdx.x + u * step, j = i + a.offset - R + 1 + d;
-            if (d < band && i < a.Sq && j >= 0 && j < a.Sk) acc[m] += (float)static_cast<const T*>(a.in)[(h * a.Sq + i) * a.Sk + j];
+            x[u] = (float)static_cast<const T*>(a.in)[(h * a.Sq + (i < a.Sq ? i : a.Sq - 1)) * a.Sk + (j < 0 ? 0 : j < a.Sk ? j : a.Sk - 1)];
+        }
+#pragma unroll
+        for (int u = 0; u < RB_ROWS; ++u) {
+            const int64_t i = blockIdx.x + u * step, j = i + a.offset - R + 1 + d;
+            acc[m] += d < band && i < a.Sq && j >= 0 && j < a.Sk ? x[u] : 0.f;
         }
     }
 #pragma unroll
