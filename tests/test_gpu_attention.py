@@ -317,6 +317,34 @@ def test_attention_position_gradient_is_as_exact_as_the_scores(t):
     assert near < far and near <= 1.5 * torch.finfo(t).eps / 2, (float(near), float(far))
 
 
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+@pytest.mark.parametrize("Sq,Sk,D", [(150, 333, 64), (50, 50, 16), (260, 260, 128), (1, 700, 80), (90, 90, 20)])
+def test_attention_with_a_position_table_rounds_its_output_once(t, Sq, Sk, D):
+    """P is carried in two pieces there (u^2 of it is lost), so of the reference's bound the term u (P |v|) becomes u^2 (P |v|)."""
+    from recboard_amd import ops
+    u = torch.finfo(t).eps / 2
+    q, k, v, _ = make(2, 4, 2, Sq, Sk, D, t, seed=Sk)
+    for causal in (False, True):
+        how = dict(rel(4, t, 32, 40), causal=causal)
+        want, tol = reference(q, k, v, **how)["out"]
+        tol = tol - (u - u * u) * reference(q, k, v.abs(), **how)["out"][0]
+        for train in (False, True):
+            out = ops.attention_fwd(q, k, v, need_backward=train, **how)[0]
+            assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("t", [torch.bfloat16, torch.float16], ids=str)
+def test_attention_position_gradient_is_off_by_its_last_rounding(t):
+    """Long rows and few buckets: the last rounding is u of each value at most; a tenth of that is left for the 32-bit sums and u^2 in delta."""
+    from recboard_amd import ops
+    q, k, v, dout = make(2, 1, 1, 2050, 2050, 32, t)
+    how = rel(1, t, 32, 64)
+    out, stats = ops.attention_fwd(q, k, v, **how)
+    got = ops.attention_bwd(dout, q, k, v, out, stats, **how)[3].double()
+    want = reference(q, k, v, dout=dout, **how)["dtable"][0]
+    assert (got - want).norm() <= 1.1 * torch.finfo(t).eps / 2 * want.norm()
+
+
 @pytest.mark.parametrize("R", [24, 40, 100])
 def test_attention_with_the_position_bias_run_to_run(R):
     q, k, v, _ = make(1, 4, 2, 150, 333, 64, torch.bfloat16)
