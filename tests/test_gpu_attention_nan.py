@@ -1,0 +1,67 @@
+"""GPU: attention where a NaN lies in a place that a row may see: that row's results are NaN, whatever way its keys are cut into parts, and no other
+row's results change."""
+import pytest
+import torch
+
+from test_gpu_attention import TYPES, make, reference
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("B,H,Hkv,Sq,Sk,D", [(2, 4, 2, 1, 1000, 64), (1, 8, 2, 1, 3001, 128), (2, 2, 2, 3, 700, 20), (1, 2, 2, 150, 900, 64), (2, 4, 2, 1, 60, 64), (2, 4, 2, 70, 60, 64)],
+                         ids=lambda x: str(x))
+def test_nan_in_a_row_of_q_stays_in_that_row(t, B, H, Hkv, Sq, Sk, D):
+    """Long caches are cut into parts and joined, short ones are not: the answer is the same either way."""
+    from recboard_amd import ops
+    q, k, v, _ = make(B, H, Hkv, Sq, Sk, D, t)
+    clean, stats = ops.attention_fwd(q, k, v)
+    q2 = q.clone()
+    q2[0, 1, Sq - 1, D // 2] = NAN
+    out, st = ops.attention_fwd(q2, k, v)
+    hit = torch.zeros(B, H, Sq, dtype=torch.bool, device="cuda")
+    hit[0, 1, Sq - 1] = True
+    assert out[hit].isnan().all()
+    # the neighbours in a tile may be made again row by row: another order of the same sums, so the definition's own bound
+    value, tol = reference(q, k, v)["out"]
+    assert ((out.double() - value).abs() <= tol)[~hit].all()
+    assert torch.isfinite(st[:2][:, ~hit]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("Sq,Sk,D,first,last", [(1, 1000, 64, 0, 128), (1, 3001, 128, 2900, 3001), (1, 3001, 128, 0, 3001), (3, 700, 20, 128, 256), (150, 900, 64, 0, 300),
+                                                (1, 60, 64, 0, 60)])
+def test_nan_in_every_key_of_a_stretch_reaches_the_rows_that_see_it(t, Sq, Sk, D, first, last):
+    from recboard_amd import ops
+    q, k, v, _ = make(2, 4, 2, Sq, Sk, D, t)
+    clean, stats = ops.attention_fwd(q, k, v)
+    k2 = k.clone()
+    k2[0, 0, first:last] = NAN
+    out, st = ops.attention_fwd(q, k2, v)
+    assert out[0, :2].isnan().all()
+    assert torch.equal(out[0, 2:], clean[0, 2:]) and torch.equal(out[1], clean[1]) and torch.equal(st[:2, 1], stats[:2, 1])
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_nan_in_a_part_whose_other_scores_are_negligible(t):
+    """The part's weight in the join is exp(-640) = 0: it is still not a part that saw nothing."""
+    from recboard_amd import ops
+    q, k, v = torch.ones(1, 1, 1, 64, device="cuda", dtype=t), torch.zeros(1, 1, 1000, 64, device="cuda", dtype=t), torch.ones(1, 1, 1000, 64, device="cuda", dtype=t)
+    k[:, :, :128] = -10.0
+    # 872 equal terms, exact in 32 bits; one rounding of 1 / 872 and one of the product, 2^-24 each (rounded to 16 bits: 1 itself)
+    assert ((ops.attention_fwd(q, k, v, scale=1.0)[0].double() - 1).abs() <= 2.0 ** -23).all()
+    k[:, :, 7] = NAN
+    assert ops.attention_fwd(q, k, v, scale=1.0)[0].isnan().all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_rows_and_parts_that_see_nothing_stay_zero_beside_nan(t):
+    from recboard_amd import ops
+    q, k, v, _ = make(3, 4, 2, 1, 1000, 64, t)
+    lens = torch.tensor([0, 1000, 100], device="cuda")
+    k[0], v[0], k[2, :, 100:], v[2, :, 100:] = NAN, NAN, NAN, NAN
+    q[0] = NAN
+    out, st = ops.attention_fwd(q, k, v, key_lengths=lens)
+    assert not out[0].any() and (st[0, 0] == -float("inf")).all() and not st[1, 0].any()
+    assert torch.isfinite(out[1:]).all() and torch.isfinite(st[:2, 1:]).all()
