@@ -760,7 +760,7 @@ int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t b
  * mask_kind 1: one byte a place, 0 = shut;  2 / 3 / 4: added to the score, fp32 / bf16 / fp16, -inf = shut.
  * bias = table[bucket_map[clip(j - (o + i), -R, R) + R], h] (re_relative_bias_fwd; table [buckets, Hq], NULL: none; R = max_distance).
  * A key that is shut for a row has no part in it, whatever k and v hold there.  A row that sees no key: out 0, stats (-inf, 0), no
- * gradients.
+ * gradients.  A NaN that a row sees makes its out and the sum of its stats NaN, and the gradients that it has a part in.
  * The rows of k and v behind key_lengths[b] are not read.  scale > 0. */
 typedef struct re_attention {
     const void *q, *k, *v;

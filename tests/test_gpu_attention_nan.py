@@ -3,7 +3,7 @@ row's results change."""
 import pytest
 import torch
 
-from test_gpu_attention import TYPES, make, reference
+from test_gpu_attention import TYPES, make, reference, rel
 
 pytestmark = pytest.mark.gpu
 NAN = float("nan")
@@ -65,3 +65,58 @@ def test_rows_and_parts_that_see_nothing_stay_zero_beside_nan(t):
     out, st = ops.attention_fwd(q, k, v, key_lengths=lens)
     assert not out[0].any() and (st[0, 0] == -float("inf")).all() and not st[1, 0].any()
     assert torch.isfinite(out[1:]).all() and torch.isfinite(st[:2, 1:]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("Sq,Sk,D,row,bias", [(50, 50, 16, 20, False), (150, 150, 64, 100, False), (90, 200, 20, 10, False), (300, 300, 128, 40, False), (600, 2100, 64, 3, False),
+                                              (150, 150, 64, 100, True)])
+def test_nan_in_a_row_of_q_reaches_the_gradients_of_the_keys_that_it_sees(t, Sq, Sk, D, row, bias):
+    """Causal: dq of the row itself and dk, dv of the keys up to its own place are NaN, everything else is what it is without that row's NaN."""
+    from recboard_amd import ops
+    q, k, v, dout = make(2, 2, 1, Sq, Sk, D, t)
+    how = dict(rel(2, t, 32, 40) if bias else {}, causal=True)
+    want = reference(q, k, v, dout=dout, **how)
+    q2 = q.clone()
+    q2[1, 0, row, 0] = NAN
+    out, stats = ops.attention_fwd(q2, k, v, **how)
+    dq, dk, dv, dtable = ops.attention_bwd(dout, q2, k, v, out, stats, **how)
+    hit = torch.zeros(2, 2, Sq, dtype=torch.bool, device="cuda")
+    hit[1, 0, row] = True
+    seen = torch.zeros(2, 1, Sk, dtype=torch.bool, device="cuda")
+    seen[1, 0, :Sk - Sq + row + 1] = True
+    for g, name, where in ((dq, "dq", hit), (dk, "dk", seen), (dv, "dv", seen)):
+        assert g[where].isnan().all(), name
+        value, tol = want[name]
+        assert ((g.double() - value).abs() <= tol)[~where].all(), name
+    if bias:
+        assert dtable[:, 0].isnan().any() and torch.isfinite(dtable[:, 1]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_gradients_of_rows_that_see_nothing_are_zero_whatever_they_hold(t):
+    from recboard_amd import ops
+    q, k, v, dout = make(2, 2, 2, 70, 70, 64, t)
+    mask = torch.ones(2, 1, 70, 70, dtype=torch.bool, device="cuda")
+    mask[0, :, 5] = False
+    want = reference(q, k, v, dout=dout, mask=mask)
+    q[0, :, 5] = NAN
+    out, stats = ops.attention_fwd(q, k, v, mask=mask)
+    assert not out[0, :, 5].any()
+    for g, name in zip(ops.attention_bwd(dout, q, k, v, out, stats, mask=mask), ("dq", "dk", "dv")):
+        value, tol = want[name]
+        assert ((g.double() - value).abs() <= tol).all(), name
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("Sq,Sk", [(1, 60), (1, 1000), (70, 60), (150, 900)])
+def test_statistics_of_a_row_whose_scores_are_nan_add_up_to_nan(t, Sq, Sk):
+    """... and not to those of a row that sees nothing, -inf and 0."""
+    from recboard_amd import ops
+    q, k, v, _ = make(2, 4, 2, Sq, Sk, 64, t)
+    q[1, 2, 0, 3] = NAN
+    k[0, 0] = NAN
+    st = ops.attention_fwd(q, k, v)[1]
+    hit = torch.zeros(2, 4, Sq, dtype=torch.bool, device="cuda")
+    hit[1, 2, 0] = True
+    hit[0, :2] = True
+    assert (st[0] + st[1])[hit].isnan().all() and torch.isfinite(st[:2][:, ~hit]).all()
