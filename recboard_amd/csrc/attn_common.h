@@ -278,30 +278,33 @@ __device__ __forceinline__ void load_lines(const args& a, int h0, int heads, flo
 // Does the mask depend on the key alone (within a sequence)?  Then a tile's part of it is one bit a key.
 __device__ __forceinline__ bool mask_by_key(const args& a) { return a.mkind == 1 && a.ms[1] == 0 && a.ms[2] == 0; }
 
-// One score, outside the matrix path: raw = q . k; -> the score, vis = false where the row may not see the key
-__device__ __forceinline__ float score_of(const args& a, float raw, int b, int h, int i, int j, int len, int off, const float* line, bool& vis) {
-    vis = j < len && !(a.causal && j > off + i);
-    float s = raw * a.scale;
-    if (!vis) return -ATTN_INF;
-    if (a.table && line) s += line[clip_distance(j - (off + i), a.R) + a.R];
-    if (a.mkind) {
-        const float m = mask_add(a, b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + j * a.ms[3]);
-        if (m == -ATTN_INF) vis = false;
-        s += m;
-    }
-    return vis ? s : -ATTN_INF;
-}
-// ... with the bias straight from its table
-__device__ __forceinline__ float score_from_table(const args& a, float raw, int b, int h, int i, int j, int len, int off, bool& vis) {
-    const float s = score_of(a, raw, b, h, i, j, len, off, nullptr, vis);
-    if (!vis || !a.table) return s;
-    return s + rb_entry(a.table, a.tdtype, a.map, clip_distance(j - (off + i), a.R) + a.R, a.buckets, a.Hq, h);
-}
 template <class T>
 __device__ __forceinline__ float dot_rows(const T* x, const T* y, int D) {
     float s = 0.f;
     for (int d = 0; d < D; ++d) s += (float)x[d] * (float)y[d];
     return s;
+}
+// One score, outside the matrix path, of query row q and key row k; vis = false, and neither row touched, where the row may not see the key
+template <class T>
+__device__ __forceinline__ float score_of(const args& a, const T* q, const T* k, int b, int h, int i, int j, int len, int off, const float* line, bool& vis) {
+    vis = j < len && !(a.causal && j > off + i);
+    if (!vis) return -ATTN_INF;
+    float m = 0.f;
+    if (a.mkind) {
+        m = mask_add(a, b * a.ms[0] + h * a.ms[1] + i * a.ms[2] + j * a.ms[3]);
+        vis = m != -ATTN_INF;
+        if (!vis) return -ATTN_INF;
+    }
+    float s = dot_rows(q, k, a.D) * a.scale;
+    if (a.table && line) s += line[clip_distance(j - (off + i), a.R) + a.R];
+    return a.mkind ? s + m : s;
+}
+// ... with the bias straight from its table
+template <class T>
+__device__ __forceinline__ float score_from_table(const args& a, const T* q, const T* k, int b, int h, int i, int j, int len, int off, bool& vis) {
+    const float s = score_of(a, q, k, b, h, i, j, len, off, nullptr, vis);
+    if (!vis || !a.table) return s;
+    return s + rb_entry(a.table, a.tdtype, a.map, clip_distance(j - (off + i), a.R) + a.R, a.buckets, a.Hq, h);
 }
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

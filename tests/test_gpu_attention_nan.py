@@ -120,3 +120,28 @@ def test_statistics_of_a_row_whose_scores_are_nan_add_up_to_nan(t, Sq, Sk):
     hit[1, 2, 0] = True
     hit[0, :2] = True
     assert (st[0] + st[1])[hit].isnan().all() and torch.isfinite(st[:2][:, ~hit]).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("D", [64, 20])
+def test_keys_behind_a_length_take_no_gradient_where_rows_are_made_again(t, D):
+    """A tile that holds the length's end, a NaN in front of it, shut for every row but one (which sends the whole tile to the row-by-row form), and NaN
+    behind: a row behind is not read there, its gradient is 0."""
+    from recboard_amd import ops
+    q, k, v, dout = make(2, 2, 1, 90, 200, D, t)
+    lens = torch.tensor([77, 200], device="cuda")
+    mask = torch.ones(2, 1, 90, 200, dtype=torch.bool, device="cuda")
+    mask[0, :, 1:, 70] = False
+    how = {"mask": mask, "key_lengths": lens}
+    want = reference(q, k, v, dout=dout, **how)
+    k, v = k.clone(), v.clone()
+    k[0, :, 70], v[0, :, 70], k[0, :, 77:], v[0, :, 77:] = NAN, NAN, NAN, NAN
+    out, stats = ops.attention_fwd(q, k, v, **how)
+    dq, dk, dv, _ = ops.attention_bwd(dout, q, k, v, out, stats, **how)
+    assert not dk[0, :, 77:].any() and not dv[0, :, 77:].any()
+    assert dq[0, :, 0].isnan().all() and torch.isfinite(dq[0, :, 1:]).all() and torch.isfinite(dq[1]).all()
+    for g, name in ((dk, "dk"), (dv, "dv")):                    # the row that saw the NaN has a part in every key of the length
+        value, tol = want[name]
+        assert g[0, :, :77].isnan().all() and ((g.double() - value).abs() <= tol)[1].all(), name
+    value, tol = want["dq"]
+    assert ((dq.double() - value).abs() <= tol)[0, :, 1:].all()
