@@ -753,7 +753,7 @@ int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t b
  * largest, or at most 8 log 2 below it) and the log of its sum of exp(score - m): their sum is the log of the softmax's denominator, and apart
  * they serve rows of any magnitude.
  * q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], Hkv a divisor of Hq (query head h reads key head h / (Hq / Hkv)), any batch / head / row
- * strides (in elements, 0 for a broadcast one), D adjacent elements in a row, 1 <= D <= 128.
+ * strides (in elements, 0 for a broadcast one, negative ones too), D adjacent elements in a row, 1 <= D <= 128.
  * The keys that query i of sequence b may see: j < key_lengths[b] (DEVICE int64 [B], optional; values outside [0, Sk] are clipped), with
  * `causal` also j <= o + i, and the mask's; o = q_offsets[b] (DEVICE int64 [B]) or, when NULL, q_offset: the position of query 0 among
  * the keys.  mask (optional) has four strides (batch, query head, query, key; 0 where it is broadcast) and is

@@ -419,7 +419,8 @@ struct attn_tensor {
     const void* p;
     const int64_t* stride;
 };
-// every row of every tensor starts on 16 bytes and is whole 16-byte chunks, and rows are not gigabytes apart
+// every row of every tensor starts on 16 bytes and is whole 16-byte chunks, and rows follow each other upwards and are not gigabytes apart (what is not
+// so goes through the form that reads element by element at 64-bit addresses)
 static inline bool attn_aligned(const attn::args& a, int32_t dtype, std::initializer_list<attn_tensor> ts) {
     const int64_t epc = 16 / (int64_t)re_dtype_size(dtype);
     if (a.D % epc) return false;
@@ -427,7 +428,7 @@ static inline bool attn_aligned(const attn::args& a, int32_t dtype, std::initial
         if (reinterpret_cast<uintptr_t>(t.p) & 15) return false;
         for (int x = 0; x < 3; ++x)
             if (t.stride[x] % epc) return false;
-        if (t.stride[2] > (1 << 22)) return false;      // (a tile's rows lie within 2^31 bytes: 32-bit offsets)
+        if (t.stride[2] < 0 || t.stride[2] > (1 << 22)) return false;      // (a tile's rows lie within 2^31 bytes of its first: unsigned 32-bit offsets)
     }
     return true;
 }
