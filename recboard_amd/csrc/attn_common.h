@@ -218,6 +218,10 @@ __device__ __forceinline__ typename mm<T>::frag reg_frag(const f32x16& x, int s)
 }
 template <class T>
 constexpr int frags_of_block() { return sizeof(T) == 4 ? 4 : 2; }
+// fp16 has its eleven bits between 2^-14 and 2^16 only (bf16 has fp32's range), and what is rounded to it here can be of any size: it is multiplied by a
+// power of two first, and the product's fp32 sums by its inverse in the end
+template <class T>
+constexpr bool narrow() { return re_type<T>::CODE == RE_F16; }
 
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32, 64); }
 __device__ __forceinline__ int row_of(int r, int half) { return 8 * (r >> 2) + 4 * half + (r & 3); }
