@@ -366,11 +366,20 @@ __device__ __forceinline__ void apply_keys(const args& a, f32x16& s, int b, int 
 }
 // 2^x as the one instruction: x <= 8 here, and below -126 the result is taken as 0 (the library's form pays four more instructions for denormals)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// exp(s - m) of a block's score; mu: m in natural units (MOD) or m * scale * log2 e of the products' units
-template <bool MOD>
+// A row's exponentials, and with them its sum and its output until it is divided by the sum, are 2^p_lift times exp(s - m).  fp16: the reference may lag by
+// 2^8 (attn_fwd.inc), so 2^7 more is what fits, and a key has its eleven bits down to 2^-21 of the reference's (64 x 700 x 128, a first key
+// that takes nearly all and adds nothing, the others about 2^-19 of it: the output was off by 1.2e-3 of its norm, its own rounding is 2e-4); the other
+// types need none.
+template <class T>
+constexpr float p_lift() { return narrow<T>() ? 7.f : 0.f; }
+template <class T>
+constexpr float p_drop() { return narrow<T>() ? 0x1p-7f : 1.f; }
+// 2^lift exp(s - m) of a block's score; mu: m in natural units (MOD) or m * scale * log2 e - lift, of the products' units
+template <class T, bool MOD>
 __device__ __forceinline__ float exp_of(float s, float mu, float c1) {
-    if constexpr (MOD) return exp2_fast((s - mu) * ATTN_LOG2E);
-    else return exp2_fast(s * c1 - mu);
+    if constexpr (!MOD) return exp2_fast(s * c1 - mu);
+    else if constexpr (narrow<T>()) return exp2_fast((s - mu) * ATTN_LOG2E + p_lift<T>());
+    else return exp2_fast((s - mu) * ATTN_LOG2E);
 }
 // May anything see key j (length, by-key mask)?  Not 0: yes.  A wave's answers for 64 keys are the bits of apply_keys; asked for a tile ahead, and
 // kept as the byte that was loaded, so that the load is not waited for before it is used.

@@ -102,3 +102,24 @@ def test_value_gradients_of_keys_with_small_probabilities(Sq, Sk):
     value, squares, _ = want
     off = (dv.double() - value).norm(dim=3)
     assert (off <= (value.half().double() - value).norm(dim=3) + 4 * U * squares.sum(3).sqrt()).all()
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("Sq,Sk,D", [(150, 2048, 64), (64, 700, 128), (1, 3000, 64), (3, 1500, 20), (700, 700, 16)])
+def test_rows_with_one_key_far_above_the_others(Sq, Sk, D, bias):
+    """The first key takes nearly all of every row and has the value 0 (what a trained causal model does with its first token): the output is
+    made of the others' probabilities, about exp(-13) = 2^-19 each."""
+    from recboard_amd import ops
+    q, k, v, dout = make(1, 2, 2, Sq, Sk, D, torch.float16)
+    q, k, v = q.clone(), k.clone(), v.clone()
+    q[..., 0], k[..., 0], k[:, :, 0] = 4.0, 0.0, 0.0
+    k[:, :, 0, 0] = 13.0 / 4.0 * math.sqrt(D)
+    v[:, :, 0] = 0.0
+    how = {"rel_table": torch.zeros(8, 2, device="cuda"), "bucket_map": ops.relative_buckets(8, 16)} if bias else {}
+    want = parts(q, k, v, dout, D ** -0.5)
+    out, stats = ops.attention_fwd(q, k, v, **how)
+    near(out, want["out"], "out")
+    lse = (q.double() @ k.double().transpose(2, 3).contiguous() * D ** -0.5).logsumexp(3)
+    assert ((stats[0] + stats[1]).double() - lse).abs().max() < 1e-4
+    got = ops.attention_bwd(dout, q, k, v, out, stats, **how)
+    near(got[2][:, :, 1:], tuple(x[:, :, 1:] if torch.is_tensor(x) else x for x in want["dv"]), "dv")
