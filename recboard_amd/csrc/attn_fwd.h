@@ -1,4 +1,5 @@
-// The launch of attention's forward kernels, between the entry point (attn_fwd.hip) and the instances for each type (attn_fwd_*.hip).
+// The launch of attention's forward kernels, between the entry point (attn_fwd.hip) and the instances for each type, aligned and
+// not (attn_fwd_*.hip).
 #pragma once
 #include "attn_common.h"
 
@@ -21,7 +22,7 @@ struct fwd_plan {
     size_t lds, part;     // bytes of LDS; of workspace
 };
 
-template <class T>
+template <class T, bool VEC>
 int fwd_launch(const args& a, const fwd_out& f, const fwd_plan& p, hipStream_t st);
 
 }  // namespace attn

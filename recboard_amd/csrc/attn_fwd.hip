@@ -36,6 +36,11 @@ static fwd_plan make_plan(const args& a, int dtype, bool vec) {
     return p;
 }
 
+template <class T>
+static int fwd_any(const args& a, const fwd_out& f, const fwd_plan& p, hipStream_t st) {
+    return p.vec ? fwd_launch<T, true>(a, f, p, st) : fwd_launch<T, false>(a, f, p, st);
+}
+
 }  // namespace attn
 
 extern "C" size_t re_attention_fwd_workspace_bytes(const re_attention* d) {
@@ -60,7 +65,6 @@ extern "C" int re_attention_fwd(const re_attention* d, void* out, const int64_t*
                           attn_order((int64_t)a.B * p.heads, (int64_t)p.tiles * p.splits, p.pg > 1 ? 1 : a.group), p.splits, p.tiles, p.heads, p.pg};
     re_clear_error();
     hipStream_t st = (hipStream_t)stream;
-    const int r = d->dtype == RE_F32 ? attn::fwd_launch<float>(a, f, p, st) : d->dtype == RE_BF16 ? attn::fwd_launch<re_bf16>(a, f, p, st)
-                                                                                              : attn::fwd_launch<re_f16>(a, f, p, st);
+    const int r = d->dtype == RE_F32 ? attn::fwd_any<float>(a, f, p, st) : d->dtype == RE_BF16 ? attn::fwd_any<re_bf16>(a, f, p, st) : attn::fwd_any<re_f16>(a, f, p, st);
     return r != RE_OK ? r : re_launch_status();
 }

@@ -1,3 +1,3 @@
 #include "attn_fwd.inc"
 
-template int attn::fwd_launch<re_bf16>(const args&, const fwd_out&, const fwd_plan&, hipStream_t);
+template int attn::fwd_launch<re_bf16, true>(const args&, const fwd_out&, const fwd_plan&, hipStream_t);

@@ -1,3 +1,3 @@
 #include "attn_fwd.inc"
 
-template int attn::fwd_launch<float>(const args&, const fwd_out&, const fwd_plan&, hipStream_t);
+template int attn::fwd_launch<float, true>(const args&, const fwd_out&, const fwd_plan&, hipStream_t);
