@@ -93,7 +93,7 @@ struct tile {
 // waited for in the middle of the one before, which a kernel of two waves a SIMD hides and a stream over a cache does not.
 __device__ __forceinline__ void to_lds(const void* base, uint32_t at, const void* lds) {
     const uint32_t to = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)lds;
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" : : "s"(__builtin_amdgcn_readfirstlane(to)), "v"(at), "s"(base) : "memory", "m0");
 }
 
 // ROWS x DP elements of a tensor into a tile, in two steps: fetch() starts the loads, land() ends them in LDS; a barrier that waits for

@@ -29,3 +29,18 @@ def spills(tmp_path_factory):
 @pytest.mark.parametrize("D,wq,wk,table,most", FORMS)
 def test_aligned_forms_with_a_mask_or_a_table_keep_their_registers(spills, D, wq, wk, table, most):
     assert spills[D, wq, wk, table] <= most
+
+
+def test_inline_assembly_that_writes_m0_says_so():
+    """A loader of LDS addresses its destination through m0; the compiler may keep a value of its own there unless the statement names it."""
+    wrote = 0
+    for name in sorted(os.listdir(os.path.join(ROOT, "recboard_amd", "csrc"))):
+        if not name.endswith((".h", ".inc", ".hip")):
+            continue
+        with open(os.path.join(ROOT, "recboard_amd", "csrc", name)) as f:
+            src = f.read()
+        for m in re.finditer(r'asm volatile\((.*?)\);', src, re.S):
+            if re.search(r"\bs_\w+ m0,", m.group(1)):
+                wrote += 1
+                assert '"m0"' in m.group(1).rsplit(":", 1)[1], (name, m.group(0))
+    assert wrote
