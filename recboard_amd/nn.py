@@ -127,17 +127,18 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, residual=None):
     return _R.add_layer_norm(x, residual, weight, bias, float(eps))[:2]
 
 
-class LayerNorm(torch.nn.Module):
-    """Drop-in for torch.nn.LayerNorm(size, eps, elementwise_affine, bias) over the last dimension; forward(x, residual) -> (y, x + residual)."""
-
-    def __init__(self, size, eps=1e-5, elementwise_affine=True, bias=True, device=None, dtype=None):
-        super().__init__()
-        self.size, self.eps = int(size), eps
-        self.weight = torch.nn.Parameter(torch.ones(self.size, device=device, dtype=dtype)) if elementwise_affine else None
-        self.bias = torch.nn.Parameter(torch.zeros(self.size, device=device, dtype=dtype)) if elementwise_affine and bias else None
+class LayerNorm(torch.nn.LayerNorm):
+    """torch.nn.LayerNorm (its arguments, names and class, over one or several last dimensions) on the engine; forward(x, residual) -> (y, x + residual)."""
 
     def forward(self, x, residual=None):
-        return layer_norm(x, self.weight, self.bias, self.eps, residual)
+        n = len(self.normalized_shape)
+        if tuple(x.shape[-n:]) != self.normalized_shape:
+            raise ValueError(f"recengine: layer norm over {self.normalized_shape} of a tensor {tuple(x.shape)}")
+        if n == 1:
+            return layer_norm(x, self.weight, self.bias, self.eps, residual)
+        one = lambda t, at: None if t is None else t.flatten(at)  # noqa: E731
+        y = layer_norm(one(x, -n), one(self.weight, 0), one(self.bias, 0), self.eps, one(residual, -n))
+        return y.view(x.shape) if residual is None else (y[0].view(x.shape), y[1].view(x.shape))
 
 
 def relative_bias(table, bucket_map, queries, keys, offset=None):
