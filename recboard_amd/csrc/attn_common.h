@@ -315,6 +315,10 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
+// The row-by-row forms stop where every sum is NaN, which no further term changes: a batch that is NaN throughout would otherwise be made again place by
+// place (2 x 16 x 4096 x 128, all of q NaN, training: 536 ms)
+template <class... F>
+__device__ __forceinline__ bool all_nan(bool live, F... v) { return __all(!live || (... && (v != v))); }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) < ATTN_INF); }
 
 // s[r] += the bias at distance d0 + SIGN * row_of(r)

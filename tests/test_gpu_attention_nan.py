@@ -145,3 +145,45 @@ def test_keys_behind_a_length_take_no_gradient_where_rows_are_made_again(t, D):
         assert g[0, :, :77].isnan().all() and ((g.double() - value).abs() <= tol)[1].all(), name
     value, tol = want["dq"]
     assert ((dq.double() - value).abs() <= tol)[0, :, 1:].all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("Sq,Sk,D", [(2048, 2048, 128), (1, 5000, 64), (70, 300, 20)])
+def test_a_batch_that_is_nan_throughout(t, Sq, Sk, D):
+    """Every row is made again; each stops at its first keys."""
+    from recboard_amd import ops
+    q, k, v, dout = make(1, 8, 2, Sq, Sk, D, t)
+    for poison in ("q", "k", "dout"):
+        x = {"q": q.clone(), "k": k.clone(), "v": v, "dout": dout.clone()}
+        x[poison].fill_(NAN)
+        out, stats = ops.attention_fwd(x["q"], x["k"], x["v"], causal=True)
+        dq, dk, dv, _ = ops.attention_bwd(x["dout"], x["q"], x["k"], x["v"], out, stats, causal=True)
+        assert dq.isnan().all() and dk.isnan().all() and dv.isnan().all()
+        assert out.isnan().all() if poison != "dout" else torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("D", [40, 128])
+def test_nan_in_single_columns_of_v_stays_in_them(t, D):
+    """A row is made again to its end while any of its sums is not NaN."""
+    from recboard_amd import ops
+    q, k, v, dout = make(1, 2, 1, 90, 300, D, t)
+    for cols in (range(0, 1), range(D // 2, D), range(0, D - 1)):
+        cols = list(cols)
+        rest = [c for c in range(D) if c not in cols]
+        v2 = v.clone()
+        v2[:, :, 3:70, cols] = NAN
+        out, _ = ops.attention_fwd(q, k, v2)
+        value, tol = reference(q, k, v)["out"]
+        assert out[..., cols].isnan().all() and ((out.double() - value).abs() <= tol)[..., rest].all()
+        one = ops.attention_fwd(q[:, :, :1], k, v2)[0]
+        assert one[..., cols].isnan().all() and torch.isfinite(one[..., rest]).all()
+    dout2 = dout.clone()
+    dout2[:, :, 5:9, 0] = NAN                                     # delta of those rows is NaN: dq of the rows, dk everywhere, dv in that column
+    out, stats = ops.attention_fwd(q, k, v)
+    dq, dk, dv, _ = ops.attention_bwd(dout2, q, k, v, out, stats)
+    want = reference(q, k, v, dout=dout)
+    rows = torch.ones(90, dtype=torch.bool, device="cuda")
+    rows[5:9] = False
+    assert dq[:, :, ~rows].isnan().all() and dk.isnan().all() and dv[..., 0].isnan().all()
+    assert ((dq.double() - want["dq"][0]).abs() <= want["dq"][1])[:, :, rows].all() and ((dv.double() - want["dv"][0]).abs() <= want["dv"][1])[..., 1:].all()
