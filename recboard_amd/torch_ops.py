@@ -390,7 +390,8 @@ fm_bag.register_autograd(_bag_bwd, setup_context=_bag_setup)
 
 
 # ---- the operators of a transformer block (fp32 / bf16 / fp16): norm, position bias, attention.  A gradient of an output that nothing used
-#      arrives as None (not as a tensor of zeros), so that the residual form does not read one.
+#      arrives as None (not as a tensor of zeros), so that the residual form does not read one.  The statistics (mean, rstd, stats) carry no gradient
+#      and say so: they do not require one.
 def _c(t):
     return None if t is None else t.contiguous()
 
@@ -436,6 +437,7 @@ def _(dy, s, weight, mean, rstd, dsum):
 def _ln_setup(ctx, inputs, output):
     x, weight, bias, eps = inputs
     ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1], output[2])
     ctx.save_for_backward(x, weight, output[1], output[2])
     ctx.bias_type = None if bias is None else bias.dtype
 
@@ -455,6 +457,7 @@ layer_norm.register_autograd(_ln_bwd, setup_context=_ln_setup)
 def _aln_setup(ctx, inputs, output):
     x, residual, weight, bias, eps = inputs
     ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[2], output[3])
     ctx.save_for_backward(weight, output[1], output[2], output[3])
     ctx.bias_type = None if bias is None else bias.dtype
 
@@ -547,6 +550,7 @@ def _(dout, q, k, v, out, stats, scale, causal, mask, key_lengths, q_offsets, q_
 def _attn_setup(ctx, inputs, output):
     q, k, v, scale, causal, mask, key_lengths, q_offsets, q_offset, table, bucket_map, need_backward = inputs
     ctx.set_materialize_grads(False)
+    ctx.mark_non_differentiable(output[1])
     ctx.save_for_backward(q, k, v, output[0], output[1], mask, key_lengths, q_offsets, table, bucket_map)
     ctx.scale, ctx.causal, ctx.q_offset = scale, causal, q_offset
 
