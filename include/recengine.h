@@ -732,7 +732,8 @@ int re_scale_copy(float* dst, const float* src, float alpha, int64_t n, re_strea
 int re_layer_norm_fwd(const void* x, const void* residual, const void* weight, const void* bias, int64_t rows, int64_t D, float eps,
                       int32_t dtype, int32_t wtype, void* y, void* sum, float* mean, float* rstd, re_stream_t stream);
 /* Its backward: dx [rows, D] = the gradient of s (= of x and of residual), `dsum` (may be NULL) the gradient that reaches s on another
- * way, added in; dweight / dbias [D] of type `wtype` (either may be NULL).  s: x of a call without residual, else its `sum`. */
+ * way, added in; dweight / dbias [D] of type `wtype` (either may be NULL).  s: x of a call without residual, else its `sum` (in a 16-bit type as
+ * rounded there, while the forward normalised the unrounded sum: rows whose mean is far larger than their spread lose u |s| / spread in dweight). */
 size_t re_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t D);
 int re_layer_norm_bwd(const void* dy, const void* s, const void* weight, const float* mean, const float* rstd, const void* dsum,
                       int64_t rows, int64_t D, int32_t dtype, int32_t wtype, void* dx, void* dweight, void* dbias, void* ws,
@@ -761,7 +762,8 @@ int re_relative_bias_bwd(const void* dbias, const int32_t* bucket_map, int64_t b
  * bias = table[bucket_map[clip(j - (o + i), -R, R) + R], h] (re_relative_bias_fwd; table [buckets, Hq], NULL: none; R = max_distance).
  * A key that is shut for a row has no part in it, whatever k and v hold there.  A row that sees no key: out 0, stats (-inf, 0), no
  * gradients.  A NaN that a row sees makes its out and the sum of its stats NaN, and the gradients that it has a part in.
- * The rows of k and v behind key_lengths[b] are not read.  scale > 0. */
+ * The rows of k and v behind key_lengths[b] are not read.  scale > 0.  A launch takes fewer than 2^23
+ * workgroups (B * Hq for each 128 queries begun; backward also B * Hkv for each 128 keys): RE_EUNSUPPORTED beyond, as for Sq, Sk >= 2^30, B > 2^24, Hq > 2^16. */
 typedef struct re_attention {
     const void *q, *k, *v;
     int64_t q_stride[3], k_stride[3], v_stride[3]; /* batch, head, row */

@@ -10,7 +10,9 @@
 // The backward's column sums stay in the registers of the lanes that own the columns over all rows of a workgroup; one partial row of dw and
 // one of db per workgroup go to the workspace and a second launch adds them in a fixed order (no atomics: run to run the same bits).
 // Measured: 16384 x 4096 bf16 behind a residual: forward 96 - 105 us (537 MB: 5.1 - 5.6 TB/s), backward 120 + 5 us (4.5 TB/s); a copy reaches 4.9.
-// All statistics and sums are fp32; s is rounded to the tensor's type once, for the store, while y comes from the unrounded sum.
+// All statistics and sums are fp32; s is rounded to the tensor's type once, for the store, while y comes from the unrounded sum.  The backward reads that
+// rounded s with the mean and rstd of the unrounded one (x and r again would be a fifth stream of HBM for four): xhat, and dw with it, is off by
+// up to u |s| / std of its row, u = 2^-8 (bf16) or 2^-11 (fp16): rows whose mean is far larger than their spread lose that much there.
 #include "re_types.h"
 
 namespace {

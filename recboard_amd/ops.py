@@ -1624,8 +1624,8 @@ def layer_norm_bwd(dy, s, weight, mean, rstd, dsum=None, weight_grads=True):
 
 def relative_buckets(num_buckets=32, max_distance=128, bidirectional=True, device="cuda"):
     """The bucket of every clipped distance key - query, [2 max_distance + 1] int32 (the operators' `bucket_map`): half of a side's buckets hold one
-    distance each, the others grow on a logarithmic scale up to max_distance, where the last begins; bidirectional: the upper half of the
-    buckets is for keys behind the query, otherwise those all share bucket 0.  The borders are found in whole numbers:
+    distance each, the others grow on a logarithmic scale whose next bucket would begin at max_distance (the last one holds that and all
+    beyond); bidirectional: the upper half of the buckets is for keys behind the query, otherwise those all share bucket 0.  The borders are found in whole numbers:
     bucket exact + m begins at the least n with (n / exact)^steps >= (max_distance / exact)^m."""
     side = num_buckets // 2 if bidirectional else num_buckets
     exact = side // 2
